@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("AIMET_B200_LIB") or os.path.join(_HERE, "lib", "libai
 AQ_OK = 0
 AQ_F32, AQ_F16, AQ_BF16 = 0, 1, 2
 AQ_V2_OUT_QDQ, AQ_V2_OUT_CODES = 0, 1
+AQ_ACT_NONE, AQ_ACT_RELU, AQ_ACT_GELU, AQ_ACT_GELU_TANH, AQ_ACT_SILU = 0, 1, 2, 3, 4
 AQ_PDF_SIZE = 512
 AQ_TFE_HIST_MANY = 16
 AQ_V2HIST_MAX_BINS = 4096
@@ -95,6 +96,16 @@ SIGNATURES = {
     "aq_v2hist_sqnr": (_i32, [_vp, _i32, _f64, _i32, _i32, _vp, _i32, _f64, _vp, _vp, _i64, _vp]),
     "aq_tfe_compute_encoding": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i64,
                                        _vp]),
+    "aq_align_rows": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _vp]),
+    "aq_linear_forward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _i32,
+                                 _vp]),
+    "aq_linear_grad_z_workspace_bytes": (_i64, [_i32, _i64, _i64]),
+    "aq_linear_grad_z": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "aq_linear_grad_input": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp]),
+    "aq_linear_grad_weight": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp]),
+    "aq_layer_norm_forward": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _f64, _vp]),
+    "aq_layer_norm_backward_workspace_bytes": (_i64, [_i32, _i64, _i64]),
+    "aq_layer_norm_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _vp]),
 }
 
 

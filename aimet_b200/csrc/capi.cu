@@ -674,4 +674,225 @@ int aq_v2hist_sqnr(const aq_v2hist_head_t* d_stats, int bins, double num_steps, 
                        d_workspace, workspace_bytes, (cudaStream_t) stream);
 }
 
+// ---- layers ------------------------------------------------------------------------------------------------------
+static inline bool bad_matrix(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype)
+{
+    return (rows > 0 && cols > 0 && !p) || ld < cols || ((uintptr_t) p % (dtype == AQ_F32 ? 4 : 2)) != 0;
+}
+// rows of 16-bit types have to start on 16-byte boundaries where the tensor cores read them
+static inline bool unaligned_rows(const void* p, int64_t ld, int dtype)
+{
+    return dtype != AQ_F32 && ((uintptr_t) p % 16 != 0 || ld % 8 != 0);
+}
+static inline bool bad_dtype(int dtype)
+{
+    return dtype < AQ_F32 || dtype > AQ_BF16;
+}
+static inline bool bad_mnk(int64_t m, int64_t n, int64_t k)
+{
+    return m < 0 || n < 1 || k < 1;
+}
+static inline bool huge(int64_t a, int64_t b = 1, int64_t c = 1)
+{
+    return a > INT32_MAX || b > INT32_MAX || c > INT32_MAX;
+}
+
+int aq_align_rows(const void* d_src, int64_t ld_src, void* d_dst, int64_t ld_dst, int dtype, int64_t rows, int64_t cols,
+                  void* stream)
+{
+    if (bad_dtype(dtype) || rows < 0 || cols < 1 || bad_matrix(d_src, ld_src, rows, cols, dtype) ||
+        bad_matrix(d_dst, ld_dst, rows, cols, dtype) || unaligned_rows(d_dst, ld_dst, dtype))
+        return AQ_ERR_INVALID_ARG;
+    if (huge(rows, ld_dst))
+        return AQ_ERR_TOO_LARGE;
+    return rows == 0 ? AQ_OK : align_rows(d_src, ld_src, d_dst, ld_dst, dtype, rows, cols, (cudaStream_t) stream);
+}
+
+int aq_linear_forward(const void* d_x, int64_t ldx, const void* d_w, int64_t ldw, const void* d_bias,
+                      const void* d_residual, int64_t ldr, void* d_y, int64_t ldy, void* d_z, int64_t ldz, int dtype,
+                      int64_t m, int64_t n, int64_t k, int activation, void* stream)
+{
+    if (bad_dtype(dtype) || bad_mnk(m, n, k) || activation < AQ_ACT_NONE || activation > AQ_ACT_SILU ||
+        bad_matrix(d_x, ldx, m, k, dtype) || bad_matrix(d_w, ldw, n, k, dtype) || bad_matrix(d_y, ldy, m, n, dtype) ||
+        (d_residual && bad_matrix(d_residual, ldr, m, n, dtype)) || (d_z && bad_matrix(d_z, ldz, m, n, dtype)) ||
+        bad_matrix(d_bias, 1, 0, 1, dtype) || unaligned_rows(d_x, ldx, dtype) || unaligned_rows(d_w, ldw, dtype))
+        return AQ_ERR_INVALID_ARG;
+    if (huge(m, n, k))
+        return AQ_ERR_TOO_LARGE;
+    if (m == 0)
+        return AQ_OK;
+    GemmArgs a = {};
+    a.a        = d_x;
+    a.lda      = ldx;
+    a.a_kmajor = 1;
+    a.b        = d_w;
+    a.ldb      = ldw;
+    a.b_kmajor = 1;
+    a.rows     = m;
+    a.cols     = n;
+    a.depth    = k;
+    a.bias     = d_bias;
+    a.residual = d_residual;
+    a.ldr      = ldr;
+    a.z        = d_z;
+    a.ldz      = ldz;
+    a.out      = d_y;
+    a.ldo      = ldy;
+    a.dtype    = dtype;
+    a.act      = activation;
+    return gemm(a, (cudaStream_t) stream);
+}
+
+int64_t aq_linear_grad_z_workspace_bytes(int dtype, int64_t m, int64_t n)
+{
+    if (bad_dtype(dtype) || m < 0 || n < 1)
+        return AQ_ERR_INVALID_ARG;
+    return grad_z_workspace_bytes(m, n);
+}
+
+int aq_linear_grad_z(const void* d_dy, int64_t lddy, const void* d_z, int64_t ldz, void* d_dz, int64_t lddz, void* d_dbias,
+                     int dtype, int64_t m, int64_t n, int activation, void* d_workspace, int64_t workspace_bytes,
+                     void* stream)
+{
+    if (bad_dtype(dtype) || bad_mnk(m, n, 1) || activation < AQ_ACT_NONE || activation > AQ_ACT_SILU ||
+        bad_matrix(d_dy, lddy, m, n, dtype) || (activation != AQ_ACT_NONE && bad_matrix(d_z, ldz, m, n, dtype)) ||
+        (d_dz && bad_matrix(d_dz, lddz, m, n, dtype)) || bad_matrix(d_dbias, 1, 0, 1, dtype))
+        return AQ_ERR_INVALID_ARG;
+    if (huge(m, n))
+        return AQ_ERR_TOO_LARGE;
+    if (d_dbias && (!d_workspace || (uintptr_t) d_workspace % 256 != 0 || workspace_bytes < grad_z_workspace_bytes(m, n)))
+        return AQ_ERR_WORKSPACE;
+    if (!d_dbias && (m == 0 || !d_dz))
+        return AQ_OK;
+    GradZArgs a = {};
+    a.dy        = d_dy;
+    a.lddy      = lddy;
+    a.z         = d_z;
+    a.ldz       = ldz;
+    a.dz        = d_dz;
+    a.lddz      = lddz;
+    a.db        = d_dbias;
+    a.part      = d_dbias ? (float*) d_workspace : nullptr;
+    a.rows      = m;
+    a.cols      = n;
+    a.dtype     = dtype;
+    a.act       = activation;
+    return grad_z(a, (cudaStream_t) stream);
+}
+
+int aq_linear_grad_input(const void* d_dz, int64_t lddz, const void* d_w, int64_t ldw, void* d_dx, int64_t lddx, int dtype,
+                         int64_t m, int64_t n, int64_t k, void* stream)
+{
+    if (bad_dtype(dtype) || bad_mnk(m, n, k) || bad_matrix(d_dz, lddz, m, n, dtype) || bad_matrix(d_w, ldw, n, k, dtype) ||
+        bad_matrix(d_dx, lddx, m, k, dtype) || unaligned_rows(d_dz, lddz, dtype) || unaligned_rows(d_w, ldw, dtype))
+        return AQ_ERR_INVALID_ARG;
+    if (huge(m, n, k))
+        return AQ_ERR_TOO_LARGE;
+    if (m == 0)
+        return AQ_OK;
+    GemmArgs a = {};
+    a.a        = d_dz;
+    a.lda      = lddz;
+    a.a_kmajor = 1;
+    a.b        = d_w;
+    a.ldb      = ldw;
+    a.rows     = m;
+    a.cols     = k;
+    a.depth    = n;
+    a.out      = d_dx;
+    a.ldo      = lddx;
+    a.dtype    = dtype;
+    return gemm(a, (cudaStream_t) stream);
+}
+
+int aq_linear_grad_weight(const void* d_dz, int64_t lddz, const void* d_x, int64_t ldx, void* d_dw, int64_t lddw, int dtype,
+                          int64_t m, int64_t n, int64_t k, void* stream)
+{
+    if (bad_dtype(dtype) || bad_mnk(m, n, k) || bad_matrix(d_dz, lddz, m, n, dtype) || bad_matrix(d_x, ldx, m, k, dtype) ||
+        bad_matrix(d_dw, lddw, n, k, dtype) || unaligned_rows(d_dz, lddz, dtype) || unaligned_rows(d_x, ldx, dtype))
+        return AQ_ERR_INVALID_ARG;
+    if (huge(m, n, k))
+        return AQ_ERR_TOO_LARGE;
+    GemmArgs a = {};
+    a.a        = d_dz;
+    a.lda      = lddz;
+    a.b        = d_x;
+    a.ldb      = ldx;
+    a.rows     = n;
+    a.cols     = k;
+    a.depth    = m;
+    a.out      = d_dw;
+    a.ldo      = lddw;
+    a.dtype    = dtype;
+    return gemm(a, (cudaStream_t) stream);
+}
+
+int aq_layer_norm_forward(const void* d_x, int64_t ldx, const void* d_w, const void* d_b, void* d_y, float* d_mean,
+                          float* d_rstd, int dtype, int64_t rows, int64_t dim, double eps, void* stream)
+{
+    if (bad_dtype(dtype) || rows < 0 || dim < 1 || bad_matrix(d_x, ldx, rows, dim, dtype) ||
+        bad_matrix(d_y, dim, rows, dim, dtype) || bad_matrix(d_w, 1, 0, 1, dtype) || bad_matrix(d_b, 1, 0, 1, dtype) ||
+        (d_mean == nullptr) != (d_rstd == nullptr) || !(eps >= 0))
+        return AQ_ERR_INVALID_ARG;
+    if (huge(rows, dim))
+        return AQ_ERR_TOO_LARGE;
+    if (rows == 0)
+        return AQ_OK;
+    LayerNormArgs a = {};
+    a.x             = d_x;
+    a.ldx           = ldx;
+    a.w             = d_w;
+    a.b             = d_b;
+    a.y             = d_y;
+    a.mean          = d_mean;
+    a.rstd          = d_rstd;
+    a.rows          = rows;
+    a.dim           = dim;
+    a.eps           = (float) eps;
+    a.dtype         = dtype;
+    return norm_fwd(a, (cudaStream_t) stream);
+}
+
+int64_t aq_layer_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t dim)
+{
+    if (bad_dtype(dtype) || rows < 0 || dim < 1)
+        return AQ_ERR_INVALID_ARG;
+    return norm_bwd_workspace_bytes(rows, dim);
+}
+
+int aq_layer_norm_backward(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const void* d_w,
+                           const float* d_mean, const float* d_rstd, void* d_dx, void* d_dw, void* d_db, int dtype,
+                           int64_t rows, int64_t dim, void* d_workspace, int64_t workspace_bytes, void* stream)
+{
+    if (bad_dtype(dtype) || rows < 0 || dim < 1 || bad_matrix(d_x, ldx, rows, dim, dtype) ||
+        bad_matrix(d_dy, lddy, rows, dim, dtype) || bad_matrix(d_w, 1, 0, 1, dtype) ||
+        bad_matrix(d_dx, dim, 0, dim, dtype) || bad_matrix(d_dw, 1, 0, 1, dtype) || bad_matrix(d_db, 1, 0, 1, dtype) ||
+        (rows > 0 && (!d_mean || !d_rstd)))
+        return AQ_ERR_INVALID_ARG;
+    if (huge(rows, dim))
+        return AQ_ERR_TOO_LARGE;
+    const bool params = d_dw || d_db;
+    if (params &&
+        (!d_workspace || (uintptr_t) d_workspace % 256 != 0 || workspace_bytes < norm_bwd_workspace_bytes(rows, dim)))
+        return AQ_ERR_WORKSPACE;
+    if (!params && (rows == 0 || !d_dx))
+        return AQ_OK;
+    LayerNormGradArgs a = {};
+    a.x                 = d_x;
+    a.ldx               = ldx;
+    a.dy                = d_dy;
+    a.lddy              = lddy;
+    a.w                 = d_w;
+    a.mean              = d_mean;
+    a.rstd              = d_rstd;
+    a.dx                = rows ? d_dx : nullptr;
+    a.dw                = d_dw;
+    a.db                = d_db;
+    a.part              = params ? (float*) d_workspace : nullptr;
+    a.rows              = rows;
+    a.dim               = dim;
+    a.dtype             = dtype;
+    return norm_bwd(a, (cudaStream_t) stream);
+}
+
 }   // extern "C"

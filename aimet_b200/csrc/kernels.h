@@ -128,4 +128,77 @@ int v2hist_sqnr(const aq_v2hist_head_t* stats, int nb, double num_steps, int sym
                 const float* offsets, int num_offsets, double gamma, float* out, void* ws, int64_t ws_bytes,
                 cudaStream_t st);
 
+// ---- layers ----------------------------------------------------------------------------------------------------
+// out[i, j] = sum_k A[i, k] B[j, k]; an operand is read as rows over k (kmajor: element (i, k) at i * ld + k) or as
+// columns (element (i, k) at k * ld + i).  bias[j], z (what the activation is applied to) and residual may be null.
+struct GemmArgs
+{
+    const void* a;
+    const void* b;
+    int64_t lda, ldb;
+    int a_kmajor, b_kmajor;
+    int64_t rows, cols, depth;
+    const void* bias;
+    const void* residual;
+    int64_t ldr;
+    void* z;
+    int64_t ldz;
+    void* out;
+    int64_t ldo;
+    int dtype, act;
+};
+int gemm(const GemmArgs& a, cudaStream_t st);
+int align_rows(const void* src, int64_t ld_src, void* dst, int64_t ld_dst, int dtype, int64_t rows, int64_t cols,
+               cudaStream_t st);
+struct GradZArgs
+{
+    const void* dy;
+    int64_t lddy;
+    const void* z;   // not read when act is AQ_ACT_NONE
+    int64_t ldz;
+    void* dz;        // may be null
+    int64_t lddz;
+    void* db;        // may be null
+    float* part;     // grad_z_workspace_bytes(rows, cols); may be null with db
+    int64_t rows, cols;
+    int dtype, act;
+};
+int64_t grad_z_workspace_bytes(int64_t rows, int64_t cols);
+int grad_z(const GradZArgs& a, cudaStream_t st);
+int fold_columns(const float* part, int64_t bands, int64_t stride, int64_t cols, void* out0, void* out1, int dtype,
+                 cudaStream_t st);
+struct LayerNormArgs
+{
+    const void* x;
+    int64_t ldx;
+    const void* w;   // may be null (1)
+    const void* b;   // may be null (0)
+    void* y;         // rows are dense
+    float* mean;     // may be null, then rstd is null too
+    float* rstd;
+    int64_t rows, dim;
+    float eps;
+    int dtype;
+};
+int norm_fwd(const LayerNormArgs& a, cudaStream_t st);
+struct LayerNormGradArgs
+{
+    const void* x;
+    int64_t ldx;
+    const void* dy;
+    int64_t lddy;
+    const void* w;   // may be null (1)
+    const float* mean;
+    const float* rstd;
+    void* dx;        // may be null; rows are dense
+    void* dw;        // may be null
+    void* db;        // may be null
+    float* part;     // norm_bwd_workspace_bytes(rows, dim); may be null with dw and db
+    int64_t rows, dim;
+    int dtype;
+};
+int64_t norm_bands(int64_t rows, int64_t dim);
+int64_t norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
+int norm_bwd(const LayerNormGradArgs& a, cudaStream_t st);
+
 }   // namespace aq

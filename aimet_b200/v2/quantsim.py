@@ -24,10 +24,11 @@ import torch
 import torch.nn.functional as F
 from torch import fx, nn
 
+from . import nn as qnn
 from .encoding_analyzer import MinMaxEncodingAnalyzer, SqnrEncodingAnalyzer, TfEnhancedEncodingAnalyzer
 from .quantizer import QuantizeDequantize
 
-__all__ = ["QuantizationSimModel", "QuantizedLayer", "fold_batch_norms"]
+__all__ = ["QuantizationSimModel", "QuantizedLayer", "QuantizedLinear", "fold_batch_norms", "fuse_layers"]
 
 _LAYERS = (nn.Conv1d, nn.Conv2d, nn.Conv3d, nn.Linear)
 _RELUS = (nn.ReLU, nn.ReLU6)
@@ -58,6 +59,21 @@ class QuantizedLayer(nn.Module):
         if wq is not None:
             with wq.compute_encodings():
                 wq(self.layer.weight)
+
+
+class QuantizedLinear(QuantizedLayer):
+    """A linear layer on :func:`aimet_b200.v2.nn.linear`: the activation and the addition that follow it in the traced
+    graph arrive as arguments and run in the product's epilogue."""
+
+    def forward(self, x, residual=None, activation=None):   # pylint: disable=arguments-differ
+        wq = self.param_quantizers["weight"]
+        weight = self.layer.weight if wq is None else wq(self.layer.weight)
+        if residual is None:
+            return qnn.linear(x, weight, self.layer.bias, activation)
+        if isinstance(residual, torch.Tensor) and residual.shape == x.shape[:-1] + weight.shape[:1] and \
+                residual.dtype == x.dtype and residual.device == x.device:
+            return qnn.linear(x, weight, self.layer.bias, activation, residual)
+        return qnn.linear(x, weight, self.layer.bias, activation) + residual   # broadcast or promoted by torch
 
 
 @torch.no_grad()
@@ -96,6 +112,143 @@ def _is_relu(node: fx.Node, mods: Dict[str, nn.Module]) -> bool:
     if node.op == "call_function":
         return node.target in _RELU_FUNCS
     return node.op == "call_method" and node.target in ("relu", "relu_")
+
+
+def _has_hooks(module: nn.Module) -> bool:
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or   # pylint: disable=protected-access
+                module._backward_pre_hooks)   # pylint: disable=protected-access
+
+
+def _activation_name(node: fx.Node, mods: Dict[str, nn.Module]) -> Optional[str]:
+    """The epilogue activation that a call node stands for, or None."""
+    if node.op == "call_module":
+        m = mods.get(node.target)
+        if m is None or _has_hooks(m):
+            return None
+        if type(m) is nn.ReLU:
+            return "relu"
+        if type(m) is nn.SiLU:
+            return "silu"
+        if type(m) is nn.GELU:
+            return {"none": "gelu", "tanh": "gelu_tanh"}.get(m.approximate)
+        return None
+    if node.op == "call_method":
+        return "relu" if node.target in ("relu", "relu_") else None
+    if node.op != "call_function":
+        return None
+    if node.target in (F.relu, torch.relu, torch.relu_):
+        return "relu"
+    if node.target is F.silu:
+        return "silu"
+    if node.target is F.gelu:
+        return {"none": "gelu", "tanh": "gelu_tanh"}.get(node.kwargs.get("approximate", "none"))
+    return None
+
+
+_IN_PLACE_FUNCS = (operator.iadd, operator.isub, operator.imul, operator.itruediv, operator.ifloordiv, operator.imod,
+                   operator.ipow, operator.iand, operator.ior, operator.ixor, operator.ilshift, operator.irshift,
+                   operator.imatmul, operator.setitem)
+
+
+def _writes_in_place(node: fx.Node, mods: Dict[str, nn.Module]) -> bool:
+    if node.op == "call_module":
+        return bool(getattr(mods.get(node.target), "inplace", False))
+    if node.op == "call_method":
+        return node.target.endswith("_")
+    if node.op == "call_function":
+        return (node.target in _IN_PLACE_FUNCS or getattr(node.target, "__name__", "").endswith("_") or
+                bool(node.kwargs.get("inplace")) or "out" in node.kwargs or
+                any(a is True for a in node.args[1:]))   # F.relu(x, True) and the like
+    return False
+
+
+def _single_user(node: fx.Node) -> Optional[fx.Node]:
+    return next(iter(node.users)) if len(node.users) == 1 else None
+
+
+def fuse_layers(gm: fx.GraphModule) -> int:
+    """Puts the linear layers and layer norms of a traced model on the kernels of :mod:`aimet_b200.v2.nn`.
+
+    A quantized ``nn.Linear`` becomes a :class:`QuantizedLinear`; a ReLU, GELU or SiLU that is its only consumer, and
+    an addition of another tensor that is the only consumer of the result, move into its epilogue.  Whatever stands
+    between them -- an activation quantizer, a second consumer, a module with hooks -- keeps them apart, so the
+    placement of quantizers and what they see stay as they were.  ``nn.LayerNorm`` modules and ``F.layer_norm`` calls
+    are replaced too.  Returns the number of graph nodes that were replaced or taken in."""
+    mods = dict(gm.named_modules())
+    changed = 0
+    for node in list(gm.graph.nodes):
+        if node.op == "call_function" and node.target is F.layer_norm and "cudnn_enable" not in node.kwargs and \
+                len(node.args) <= 5:
+            kw = dict(node.kwargs)
+            if "input" in kw:
+                kw["x"] = kw.pop("input")
+            node.target, node.kwargs = qnn.layer_norm, kw
+            changed += 1
+        if node.op != "call_module":
+            continue
+        m = mods.get(node.target)
+        if type(m) is nn.LayerNorm and not _has_hooks(m):
+            new = qnn.LayerNorm.from_module(m)
+        elif type(m) is QuantizedLayer and type(m.layer) is nn.Linear and not _has_hooks(m) and not _has_hooks(m.layer):
+            new = QuantizedLinear(m.layer, None)
+            new.param_quantizers = m.param_quantizers
+            new.train(m.training)
+        else:
+            continue
+        for name, other in list(mods.items()):
+            if other is m:
+                mods[name] = new
+        parent_name, _, leaf = node.target.rpartition(".")
+        setattr(gm.get_submodule(parent_name) if parent_name else gm, leaf, new)
+        changed += 1
+    order = {node: i for i, node in enumerate(gm.graph.nodes)}
+    writers = [order[node] for node in gm.graph.nodes if _writes_in_place(node, mods)]
+    for node in list(gm.graph.nodes):
+        if node.op != "call_module" or type(mods.get(node.target)) is not QuantizedLinear or len(node.args) != 1:
+            continue
+        last = node
+        kwargs = dict(node.kwargs)
+        user = _single_user(last)
+        if "residual" not in kwargs and "activation" not in kwargs and user is not None and \
+                user.args and user.args[0] is last:
+            name = _activation_name(user, mods)
+            if name is not None:
+                kwargs["activation"] = name
+                last = user
+                user = _single_user(last)
+        if "residual" not in kwargs and user is not None and user.op == "call_function" and user.target in _ADDS and \
+                len(user.args) == 2 and not user.kwargs:
+            left, right = user.args
+            other = right if left is last else left
+            # x += linear(...) writes to x; anything written in place in between could change what the layer reads
+            mine = (order[last],) if last is not node else ()
+            quiet = not any(order[node] < w < order[user] and w not in mine for w in writers)
+            if isinstance(other, fx.Node) and other is not last and quiet and \
+                    (user.target is not operator.iadd or left is last):
+                kwargs["residual"] = other
+                last = user
+        if last is node:
+            continue
+        with gm.graph.inserting_before(last):
+            new = gm.graph.call_module(node.target, node.args, kwargs)
+        order[new] = order[last]
+        last.replace_all_uses_with(new)
+        for old in (last, *_between(node, last)):
+            gm.graph.erase_node(old)
+            changed += 1
+    gm.graph.lint()
+    gm.recompile()
+    gm.delete_all_unused_submodules()
+    return changed
+
+
+def _between(first: fx.Node, last: fx.Node) -> List[fx.Node]:
+    """The nodes of a chain from ``last`` (exclusive) back to ``first`` (inclusive)."""
+    chain, cur = [], first
+    while cur is not last:
+        chain.append(cur)
+        cur = _single_user(cur)
+    return chain[::-1]
 
 
 class QuantizationSimModel:
@@ -202,6 +355,16 @@ class QuantizationSimModel:
                 stack.enter_context(q.compute_encodings())
             with torch.no_grad():
                 forward_pass_callback(self.model, forward_pass_callback_args)
+
+    # ---- kernels for the layers ---------------------------------------------------------------------------------
+    def fuse_layers(self) -> int:
+        """Runs the linear layers and layer norms of ``sim.model`` on the kernels of :mod:`aimet_b200.v2.nn`
+        (:func:`fuse_layers`), with float32 sums in another order than torch's.  Quantizers, encodings and parameters
+        stay the same objects.  Can be called again, for instance after ``load_encodings(..., partial=False)`` removed
+        quantizers that kept a layer and its activation apart.  From then on the model needs CUDA tensors."""
+        changed = fuse_layers(self.model)
+        self.layers = {name: self.model.get_submodule(name) for name in self.layers}
+        return changed
 
     # ---- encodings on disk -------------------------------------------------------------------------------------
     def get_encodings_dict(self) -> dict:

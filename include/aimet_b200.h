@@ -498,6 +498,67 @@ int aq_v2hist_sqnr_encode_rows(const aq_v2hist_head_t* d_stats, int64_t block_st
                                int stats_dtype, double qmin, float* d_out, void* d_workspace, int64_t workspace_bytes,
                                void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Layers between the quantizers.  The reference runs its quantized layers on torch's own functions
+ * (aimet_torch/v2/nn/fake_quant.py: FakeQuantizedLinear, FakeQuantizedLayerNorm); these are the same
+ * functions with the work around the product fused into it.
+ *
+ * Matrices are row-major with a row pitch in elements (ld*, at least the row length).  All operands of a call have
+ * one dtype (AQ_F32 / AQ_F16 / AQ_BF16); products and sums are float32, each result is rounded once.  Outputs must
+ * not overlap inputs.  "Aligned" matrices: for AQ_F16 and AQ_BF16 every row has to start on a 16-byte boundary (base
+ * and pitch); aq_align_rows makes such a copy.  AQ_F32 needs no more than the alignment of a float.
+ * ---------------------------------------------------------------------------------------------- */
+typedef enum
+{
+    AQ_ACT_NONE      = 0,
+    AQ_ACT_RELU      = 1,
+    AQ_ACT_GELU      = 2, /* z / 2 * (1 + erf(z / sqrt 2)) */
+    AQ_ACT_GELU_TANH = 3, /* z / 2 * (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+    AQ_ACT_SILU      = 4  /* z / (1 + exp(-z)) */
+} aq_activation_t;
+
+/* Copies rows x cols elements from pitch ld_src to pitch ld_dst; the elements between cols and ld_dst become 0. */
+int aq_align_rows(const void* d_src, int64_t ld_src, void* d_dst, int64_t ld_dst, int dtype, int64_t rows,
+                  int64_t cols, void* stream);
+
+/* y = act(x W^T + bias) + residual; x [m, k] and W [n, k] aligned, bias [n] or NULL, residual [m, n] or NULL,
+ * y [m, n].  d_z, if not NULL, receives z = x W^T + bias [m, n] for the backward pass, rounded to dtype. */
+int aq_linear_forward(const void* d_x, int64_t ldx, const void* d_w, int64_t ldw, const void* d_bias,
+                      const void* d_residual, int64_t ldr, void* d_y, int64_t ldy, void* d_z, int64_t ldz, int dtype,
+                      int64_t m, int64_t n, int64_t k, int activation, void* stream);
+
+/* Bytes of scratch (256-byte aligned, any content) of aq_linear_grad_z. */
+int64_t aq_linear_grad_z_workspace_bytes(int dtype, int64_t m, int64_t n);
+
+/* dz = dy act'(z) [m, n] (rounded to dtype) and dbias = sum over rows of the unrounded dz [n].  d_dz or d_dbias may
+ * be NULL; d_z is not read for AQ_ACT_NONE.  m = 0 writes a zero dbias. */
+int aq_linear_grad_z(const void* d_dy, int64_t lddy, const void* d_z, int64_t ldz, void* d_dz, int64_t lddz,
+                     void* d_dbias, int dtype, int64_t m, int64_t n, int activation, void* d_workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* dx = dz W: dz [m, n] and W [n, k] aligned, dx [m, k]. */
+int aq_linear_grad_input(const void* d_dz, int64_t lddz, const void* d_w, int64_t ldw, void* d_dx, int64_t lddx,
+                         int dtype, int64_t m, int64_t n, int64_t k, void* stream);
+
+/* dW = dz^T x: dz [m, n] and x [m, k] aligned, dW [n, k].  m = 0 writes zeros. */
+int aq_linear_grad_weight(const void* d_dz, int64_t lddz, const void* d_x, int64_t ldx, void* d_dw, int64_t lddw,
+                          int dtype, int64_t m, int64_t n, int64_t k, void* stream);
+
+/* y = (x - mean) / sqrt(var + eps) * w + b over rows of dim elements (var: mean of squared differences).
+ * d_w / d_b: dim elements of dtype, or NULL for 1 / 0.  d_mean, d_rstd: one float per row for the backward pass, both
+ * or neither NULL.  y is dense [rows, dim]. */
+int aq_layer_norm_forward(const void* d_x, int64_t ldx, const void* d_w, const void* d_b, void* d_y, float* d_mean,
+                          float* d_rstd, int dtype, int64_t rows, int64_t dim, double eps, void* stream);
+
+/* Bytes of scratch (256-byte aligned, any content) of aq_layer_norm_backward. */
+int64_t aq_layer_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t dim);
+
+/* dx (dense [rows, dim]), dw and db (dim elements of dtype) from dy, the input and what the forward call left in
+ * d_mean / d_rstd.  Any of the three results may be NULL.  rows = 0 writes zero dw and db. */
+int aq_layer_norm_backward(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const void* d_w,
+                           const float* d_mean, const float* d_rstd, void* d_dx, void* d_dw, void* d_db, int dtype,
+                           int64_t rows, int64_t dim, void* d_workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

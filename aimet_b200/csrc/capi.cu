@@ -694,7 +694,8 @@ static inline bool bad_mnk(int64_t m, int64_t n, int64_t k)
 }
 static inline bool huge(int64_t a, int64_t b = 1, int64_t c = 1)
 {
-    return a > INT32_MAX || b > INT32_MAX || c > INT32_MAX;
+    const int64_t most = INT32_MAX - 256;   // a last tile still starts and ends inside an int
+    return a > most || b > most || c > most;
 }
 
 int aq_align_rows(const void* d_src, int64_t ld_src, void* d_dst, int64_t ld_dst, int dtype, int64_t rows, int64_t cols,
@@ -825,6 +826,11 @@ int aq_linear_grad_weight(const void* d_dz, int64_t lddz, const void* d_x, int64
     a.ldo      = lddw;
     a.dtype    = dtype;
     return gemm(a, (cudaStream_t) stream);
+}
+
+int aq_linear_stuck(int* h_out)
+{
+    return h_out ? gemm_stuck(h_out) : AQ_ERR_INVALID_ARG;
 }
 
 int aq_layer_norm_forward(const void* d_x, int64_t ldx, const void* d_w, const void* d_b, void* d_y, float* d_mean,

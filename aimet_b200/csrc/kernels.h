@@ -148,6 +148,8 @@ struct GemmArgs
     int dtype, act;
 };
 int gemm(const GemmArgs& a, cudaStream_t st);
+int tensor_gemm(const GemmArgs& a, cudaStream_t st);   // 16-bit operands, depth of at least 1
+int gemm_stuck(int* out);
 int align_rows(const void* src, int64_t ld_src, void* dst, int64_t ld_dst, int dtype, int64_t rows, int64_t cols,
                cudaStream_t st);
 struct GradZArgs

@@ -257,12 +257,14 @@ int grad_z(const GradZArgs& a, cudaStream_t st)
 
 int gemm(const GemmArgs& a, cudaStream_t st)
 {
-    switch (a.dtype)
+    if (a.dtype == AQ_F32)
+        return simt_dispatch<float>(a, st);
+    if (a.depth == 0)
     {
-    case AQ_F32: return simt_dispatch<float>(a, st);
-    case AQ_F16: return simt_dispatch<__half>(a, st);
-    default: return simt_dispatch<__nv_bfloat16>(a, st);
+        const cudaError_t e = cudaMemset2DAsync(a.out, (size_t) a.ldo * 2, 0, (size_t) a.cols * 2, (size_t) a.rows, st);
+        return e == cudaSuccess ? AQ_OK : cuda_fail(e);
     }
+    return tensor_gemm(a, st);
 }
 
 }   // namespace aq

@@ -594,3 +594,11 @@ def test_quantsim_fused_layers(cuda, without_activation_quantizers):
     torch.testing.assert_close(out[0][0], out[1][0], rtol=1e-4, atol=1e-4 + 4 * step)
     for a, b in zip(out[0][1] + [out[0][2]], out[1][1] + [out[1][2]]):
         assert float((a - b).norm()) <= 2e-3 * float(a.norm())
+
+
+def test_no_wait_ran_out(cuda):
+    """Runs last in this file: none of the products above gave up on a wait."""
+    import ctypes
+    from aimet_b200._lib import lib
+    out = ctypes.c_int(7)
+    assert lib.aq_linear_stuck(ctypes.byref(out)) == 0 and out.value == 0

@@ -1,9 +1,14 @@
 // The activations a linear layer can carry in its epilogue, and their slopes, in float32.
 //
 //   relu       max(z, 0)
-//   gelu       z / 2 * (1 + erf(z / sqrt 2))
-//   gelu_tanh  z / 2 * (1 + tanh(sqrt(2 / pi) * (z + 0.044715 z^3)))
-//   silu       z / (1 + exp(-z))
+//   gelu       z P(z),       P(z) = (1 + erf(z / sqrt 2)) / 2
+//   gelu_tanh  z s(2 u(z)),  u(z) = sqrt(2 / pi) (z + 0.044715 z^3), s the logistic function: (1 + tanh u) / 2 = s(2 u)
+//   silu       z s(z)
+//
+// FAST is for 16-bit results: the hardware's exponential and reciprocal (relative error near 2^-21), and for P the
+// rational approximation 7.1.26 of Abramowitz and Stegun (Handbook of Mathematical Functions; error of erf at most
+// 1.5e-7), whose exp(-z^2 / 2) is also the density that the slope needs.  The backward pass of a 16384 x 11008 bf16
+// layer is bound by instructions with erff and expf: see grad_z_kernel.
 //
 // NaN stays NaN in every value.  The slopes take their limits 0 and 1 beyond |z| = 14 (gelu; what is left of the
 // derivative is below 1e-40) or |z| = 100 (silu; below 1e-41): the formulas would form 0 * inf there.
@@ -13,61 +18,96 @@
 
 namespace aq
 {
-template <int ACT>
+template <bool FAST>
+__device__ __forceinline__ float logistic(float x)
+{
+    if constexpr (FAST)
+        return __fdividef(1.f, 1.f + __expf(-x));
+    else
+        return 1.f / (1.f + expf(-x));
+}
+
+// P(z), and exp(-z^2 / 2) for the slope
+template <bool FAST>
+__device__ __forceinline__ float normal_cdf(float z, float& e)
+{
+    if constexpr (FAST)
+    {
+        const float x = fabsf(z) * 0.70710678f;
+        const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+        float q       = fmaf(1.061405429f, t, -1.453152027f);
+        q             = fmaf(q, t, 1.421413741f);
+        q             = fmaf(q, t, -0.284496736f);
+        q             = fmaf(q, t, 0.254829592f);
+        e             = __expf(-x * x);
+        const float tail = 0.5f * q * t * e;   // P(-|z|)
+        return z > 0.f ? 1.f - tail : tail;
+    }
+    else
+    {
+        e = expf(-0.5f * z * z);
+        return 0.5f * (1.f + erff(z * 0.70710678f));
+    }
+}
+
+template <int ACT, bool FAST>
 __device__ __forceinline__ float act_value(float z)
 {
     if constexpr (ACT == AQ_ACT_RELU)
         return z < 0.f ? 0.f : z;
     else if constexpr (ACT == AQ_ACT_GELU)
-        return 0.5f * z * (1.f + erff(z * 0.70710678f));
+    {
+        float e;
+        return z * normal_cdf<FAST>(z, e);
+    }
     else if constexpr (ACT == AQ_ACT_GELU_TANH)
-        return 0.5f * z * (1.f + tanhf(0.79788456f * (z + 0.044715f * z * z * z)));
+        return z * logistic<FAST>(1.5957691f * z * fmaf(0.044715f * z, z, 1.f));
     else if constexpr (ACT == AQ_ACT_SILU)
-        return z / (1.f + expf(-z));
+        return z * logistic<FAST>(z);
     else
         return z;
 }
 
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ float act_slope(float z)
 {
     if constexpr (ACT == AQ_ACT_RELU)
         return z > 0.f ? 1.f : 0.f;
     else if constexpr (ACT == AQ_ACT_GELU)
     {
-        if (fabsf(z) > 14.f)
-            return z > 0.f ? 1.f : 0.f;
-        return 0.5f * (1.f + erff(z * 0.70710678f)) + z * expf(-0.5f * z * z) * 0.39894228f;
+        float e;
+        const float p = normal_cdf<FAST>(z, e);
+        const float s = fmaf(z * 0.39894228f, e, p);
+        return fabsf(z) > 14.f ? (z > 0.f ? 1.f : 0.f) : s;
     }
     else if constexpr (ACT == AQ_ACT_GELU_TANH)
     {
-        if (fabsf(z) > 14.f)
-            return z > 0.f ? 1.f : 0.f;
-        const float t = tanhf(0.79788456f * (z + 0.044715f * z * z * z));
-        return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456f * (1.f + 0.134145f * z * z);
+        const float z2 = z * z;
+        const float p  = logistic<FAST>(1.5957691f * z * fmaf(0.044715f, z2, 1.f));
+        const float s  = fmaf(z * p * (1.f - p), 1.5957691f * fmaf(0.134145f, z2, 1.f), p);
+        return fabsf(z) > 14.f ? (z > 0.f ? 1.f : 0.f) : s;
     }
     else if constexpr (ACT == AQ_ACT_SILU)
     {
-        if (fabsf(z) > 100.f)
-            return z > 0.f ? 1.f : 0.f;
-        const float p = 1.f / (1.f + expf(-z));
-        return p * (1.f + z * (1.f - p));
+        const float p = logistic<FAST>(z);
+        const float s = p * fmaf(z, 1.f - p, 1.f);
+        return fabsf(z) > 100.f ? (z > 0.f ? 1.f : 0.f) : s;
     }
     else
         return 1.f;
 }
 
 // dz = dy * act'(z).  A zero slope gives zero whatever dy holds (a masked infinity stays out of the sums).
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ float act_grad(float dy, float z)
 {
     if constexpr (ACT == AQ_ACT_NONE)
         return dy;
-    const float s = act_slope<ACT>(z);
+    const float s = act_slope<ACT, FAST>(z);
     return s == 0.f ? 0.f : dy * s;
 }
 
-// f.template operator()<ACT>() for the run-time value `act`; every kernel launcher below dispatches through it
+// f(std::integral_constant<int, ACT>) for the run-time value `act`
 template <typename F>
 inline int with_activation(int act, F&& f)
 {

@@ -199,7 +199,6 @@ struct LayerNormGradArgs
     int64_t rows, dim;
     int dtype;
 };
-int64_t norm_bands(int64_t rows, int64_t dim);
 int64_t norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
 int norm_bwd(const LayerNormGradArgs& a, cudaStream_t st);
 

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kSimtThreads) simt_gemm_kernel(GemmArgs a)
                 z += to_f32(((const T*) a.bias)[j]);
             if (a.z)
                 ((T*) a.z)[i * a.ldz + j] = from_f32<T>(z);
-            float y = act_value<ACT>(z);
+            float y = act_value<ACT, false>(z);
             if (a.residual)
                 y += to_f32(((const T*) a.residual)[i * a.ldr + j]);
             ((T*) a.out)[i * a.ldo + j] = from_f32<T>(y);
@@ -110,54 +110,114 @@ int simt_dispatch(const GemmArgs& a, cudaStream_t st)
 }
 
 // ------------------------------------------------------------------------------------------------
-// dz = dy act'(z) and the partial sums of db: a CTA of 8 warps takes 32 columns and every 8th row of its band per warp.
+// dz = dy act'(z) and the partial sums of db.  A thread owns VEC neighbouring columns, a warp 32 VEC of them, and the
+// 8 warps of a CTA take the rows of its band in turn, four of them in flight per thread; the sums stay in registers
+// until the band ends.  Bound by memory (dy and z in, dz out) once the slope costs few instructions: with erff and
+// expf the gelu form of a bf16 16384 x 11008 layer is bound by issue.
 // ------------------------------------------------------------------------------------------------
-template <typename T, int ACT>
+constexpr int kBandRowsAtOnce = 4;
+
+template <typename T, int ACT, int VEC>
 __global__ void __launch_bounds__(256) grad_z_kernel(GradZArgs a, int64_t band_rows)
 {
-    __shared__ float sh[8][32];
+    constexpr bool FAST = sizeof(T) == 2;
+    __shared__ float sh[8][32 * VEC + 4];
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t col  = (int64_t) blockIdx.x * 32 + lane;
+    const int64_t col  = ((int64_t) blockIdx.x * 32 + lane) * VEC;
     const int64_t row0 = (int64_t) blockIdx.y * band_rows;
     const int64_t row1 = row0 + band_rows < a.rows ? row0 + band_rows : a.rows;
-    float db = 0.f;
-    if (col < a.cols)
-        for (int64_t row = row0 + warp; row < row1; row += 8)
-        {
-            const float dy = to_f32(((const T*) a.dy)[row * a.lddy + col]);
-            const float dz = ACT == AQ_ACT_NONE ? dy : act_grad<ACT>(dy, to_f32(((const T*) a.z)[row * a.ldz + col]));
-            if (a.dz)
-                ((T*) a.dz)[row * a.lddz + col] = from_f32<T>(dz);
-            db += dz;
-        }
-    sh[warp][lane] = db;
-    __syncthreads();
-    if (warp == 0 && col < a.cols && a.part)
+    float db[VEC]      = {};
+    if (col < a.cols)   // VEC divides the number of columns
     {
-        float s = 0.f;
+        const T* dy = (const T*) a.dy + col;
+        const T* z  = (const T*) a.z + col;
+        T* dz       = (T*) a.dz + col;
+        for (int64_t row = row0 + warp; row < row1; row += 8 * kBandRowsAtOnce)
+        {
+            Pack<T, VEC> g[kBandRowsAtOnce], h[kBandRowsAtOnce];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            s += sh[i][lane];
-        a.part[(int64_t) blockIdx.y * a.cols + col] = s;
+            for (int u = 0; u < kBandRowsAtOnce; ++u)
+                if (row + 8 * u < row1)
+                {
+                    g[u] = load_pack<T, VEC>(dy + (row + 8 * u) * a.lddy);
+                    if (ACT != AQ_ACT_NONE)
+                        h[u] = load_pack<T, VEC>(z + (row + 8 * u) * a.ldz);
+                }
+#pragma unroll
+            for (int u = 0; u < kBandRowsAtOnce; ++u)
+                if (row + 8 * u < row1)
+                {
+                    Pack<T, VEC> o;
+#pragma unroll
+                    for (int c = 0; c < VEC; ++c)
+                    {
+                        float v = to_f32(g[u].v[c]);
+                        if (ACT != AQ_ACT_NONE)
+                            v = act_grad<ACT, FAST>(v, to_f32(h[u].v[c]));
+                        o.v[c] = from_f32<T>(v);
+                        db[c] += v;
+                    }
+                    if (a.dz)
+                        store_pack<T, VEC>(dz + (row + 8 * u) * a.lddz, o);
+                }
+        }
+    }
+    if (!a.part)
+        return;
+#pragma unroll
+    for (int c = 0; c < VEC; ++c)
+        sh[warp][lane * VEC + c] = db[c];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * VEC; c += 256)
+    {
+        const int64_t out = (int64_t) blockIdx.x * 32 * VEC + c;
+        if (out < a.cols)
+        {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                s += sh[i][c];
+            a.part[(int64_t) blockIdx.y * a.cols + out] = s;
+        }
     }
 }
 
-template <typename T>
-int grad_z_t(const GradZArgs& a, cudaStream_t st)
+// Bands for `ctas` column tiles: enough CTAs for 8 per SM, at least 64 rows each.
+int64_t grad_bands(int64_t rows, int64_t ctas)
 {
-    const int64_t bands     = norm_bands(a.rows, a.cols);
+    int64_t bands      = (8 * kNumSMs + ctas - 1) / ctas;
+    const int64_t most = (rows + 63) / 64;
+    bands              = bands < most ? bands : most;
+    return bands < 1 ? 1 : bands;
+}
+
+template <typename T, int VEC>
+int grad_z_v(const GradZArgs& a, cudaStream_t st)
+{
+    const int64_t ctas      = (a.cols + 32 * VEC - 1) / (32 * VEC);
+    const int64_t bands     = grad_bands(a.rows, ctas);
     const int64_t band_rows = (a.rows + bands - 1) / bands;
     const int rc            = with_activation(a.act, [&](auto act) {
-        const cudaError_t e = launch_pdl(grad_z_kernel<T, decltype(act)::value>,
-                                         dim3((unsigned) ((a.cols + 31) / 32), (unsigned) bands), 256, 0, st, a, band_rows);
+        const cudaError_t e = launch_pdl(grad_z_kernel<T, decltype(act)::value, VEC>, dim3((unsigned) ctas, (unsigned) bands),
+                                                    256, 0, st, a, band_rows);
         note_launch();
         return e == cudaSuccess ? AQ_OK : cuda_fail(e);
     });
     if (rc != AQ_OK || !a.db)
         return rc;
     return fold_columns(a.part, bands, a.cols, a.cols, a.db, nullptr, a.dtype, st);
+}
+
+template <typename T>
+int grad_z_t(const GradZArgs& a, cudaStream_t st)
+{
+    // 16 bytes per access where every row of every matrix starts on such a boundary, else element by element
+    constexpr int W = 16 / (int) sizeof(T);
+    auto fits       = [&](const void* p, int64_t ld) { return !p || ((uintptr_t) p % 16 == 0 && ld % W == 0); };
+    const bool wide = a.cols % W == 0 && fits(a.dy, a.lddy) && fits(a.dz, a.lddz) && (a.act == AQ_ACT_NONE || fits(a.z, a.ldz));
+    return wide ? grad_z_v<T, W>(a, st) : grad_z_v<T, 1>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -242,7 +302,8 @@ int fold_columns(const float* part, int64_t bands, int64_t stride, int64_t cols,
 
 int64_t grad_z_workspace_bytes(int64_t rows, int64_t cols)
 {
-    return norm_bands(rows, cols) * cols * (int64_t) sizeof(float);
+    // the number of bands falls with the number of column tiles: the widest tiles need the most
+    return grad_bands(rows, (cols + 255) / 256) * cols * (int64_t) sizeof(float);
 }
 
 int grad_z(const GradZArgs& a, cudaStream_t st)

@@ -44,22 +44,22 @@ __device__ __forceinline__ void activate(float (&v)[N], int act)
     case AQ_ACT_RELU:
 #pragma unroll
         for (int c = 0; c < N; ++c)
-            v[c] = act_value<AQ_ACT_RELU>(v[c]);
+            v[c] = act_value<AQ_ACT_RELU, true>(v[c]);
         break;
     case AQ_ACT_GELU:
 #pragma unroll
         for (int c = 0; c < N; ++c)
-            v[c] = act_value<AQ_ACT_GELU>(v[c]);
+            v[c] = act_value<AQ_ACT_GELU, true>(v[c]);
         break;
     case AQ_ACT_GELU_TANH:
 #pragma unroll
         for (int c = 0; c < N; ++c)
-            v[c] = act_value<AQ_ACT_GELU_TANH>(v[c]);
+            v[c] = act_value<AQ_ACT_GELU_TANH, true>(v[c]);
         break;
     case AQ_ACT_SILU:
 #pragma unroll
         for (int c = 0; c < N; ++c)
-            v[c] = act_value<AQ_ACT_SILU>(v[c]);
+            v[c] = act_value<AQ_ACT_SILU, true>(v[c]);
         break;
     default: break;
     }

@@ -103,7 +103,7 @@ SIGNATURES = {
     "aq_linear_grad_z": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i32, _vp, _i64, _vp]),
     "aq_linear_grad_input": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp]),
     "aq_linear_grad_weight": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp]),
-    "aq_linear_stuck": (_i32, [C.POINTER(_i32)]),
+    "aq_layers_stuck": (_i32, [C.POINTER(_i32)]),
     "aq_layer_norm_forward": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _f64, _vp]),
     "aq_layer_norm_backward_workspace_bytes": (_i64, [_i32, _i64, _i64]),
     "aq_layer_norm_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _vp]),

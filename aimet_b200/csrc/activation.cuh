@@ -18,11 +18,25 @@
 
 namespace aq
 {
+__device__ __forceinline__ float fast_rcp(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float fast_exp2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// s(x) from -x log2(e)
 template <bool FAST>
 __device__ __forceinline__ float logistic(float x)
 {
     if constexpr (FAST)
-        return __fdividef(1.f, 1.f + __expf(-x));
+        return fast_rcp(1.f + fast_exp2(-1.44269504f * x));
     else
         return 1.f / (1.f + expf(-x));
 }
@@ -33,14 +47,14 @@ __device__ __forceinline__ float normal_cdf(float z, float& e)
 {
     if constexpr (FAST)
     {
-        const float x = fabsf(z) * 0.70710678f;
-        const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-        float q       = fmaf(1.061405429f, t, -1.453152027f);
-        q             = fmaf(q, t, 1.421413741f);
-        q             = fmaf(q, t, -0.284496736f);
-        q             = fmaf(q, t, 0.254829592f);
-        e             = __expf(-x * x);
-        const float tail = 0.5f * q * t * e;   // P(-|z|)
+        // 7.1.26 at |z| / sqrt 2: p / sqrt 2 = 0.23164189, the five coefficients halved
+        const float t = fast_rcp(fmaf(0.23164189f, fabsf(z), 1.f));
+        float q       = fmaf(0.5307027145f, t, -0.7265760135f);
+        q             = fmaf(q, t, 0.7107068705f);
+        q             = fmaf(q, t, -0.142248368f);
+        q             = fmaf(q, t, 0.127414796f);
+        e             = fast_exp2(-0.72134752f * z * z);
+        const float tail = q * t * e;   // P(-|z|)
         return z > 0.f ? 1.f - tail : tail;
     }
     else
@@ -97,14 +111,15 @@ __device__ __forceinline__ float act_slope(float z)
         return 1.f;
 }
 
-// dz = dy * act'(z).  A zero slope gives zero whatever dy holds (a masked infinity stays out of the sums).
+// dz = dy * act'(z).  Where relu is off the result is zero whatever dy holds (an infinity stays out of the sums).
 template <int ACT, bool FAST>
 __device__ __forceinline__ float act_grad(float dy, float z)
 {
     if constexpr (ACT == AQ_ACT_NONE)
         return dy;
-    const float s = act_slope<ACT, FAST>(z);
-    return s == 0.f ? 0.f : dy * s;
+    if constexpr (ACT == AQ_ACT_RELU)
+        return z > 0.f ? dy : 0.f;
+    return dy * act_slope<ACT, FAST>(z);
 }
 
 // f(std::integral_constant<int, ACT>) for the run-time value `act`

@@ -828,9 +828,16 @@ int aq_linear_grad_weight(const void* d_dz, int64_t lddz, const void* d_x, int64
     return gemm(a, (cudaStream_t) stream);
 }
 
-int aq_linear_stuck(int* h_out)
+int aq_layers_stuck(int* h_out)
 {
-    return h_out ? gemm_stuck(h_out) : AQ_ERR_INVALID_ARG;
+    if (!h_out)
+        return AQ_ERR_INVALID_ARG;
+    int gemm_flag = 0, norm_flag = 0;
+    int rc = gemm_stuck(&gemm_flag);
+    if (rc == AQ_OK)
+        rc = norm_stuck(&norm_flag);
+    *h_out = gemm_flag || norm_flag;
+    return rc;
 }
 
 int aq_layer_norm_forward(const void* d_x, int64_t ldx, const void* d_w, const void* d_b, void* d_y, float* d_mean,

@@ -201,5 +201,6 @@ struct LayerNormGradArgs
 };
 int64_t norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
 int norm_bwd(const LayerNormGradArgs& a, cudaStream_t st);
+int norm_stuck(int* out);
 
 }   // namespace aq

@@ -7,10 +7,15 @@
 // against the spread); every sum is float32.  All of it is bound by memory: x is read and y written once forward, x and
 // dy read and dx written once backward.
 //
-// Rows that fit into the registers of 32 to 512 threads take the kernels that hold them there (one pass over memory);
-// longer rows take the *_loop_* kernels, which walk a row two or three times (again out of L2), and norm_param_kernel.
+// Which kernel takes a call:
+//   norm_fwd_kernel        forward, few rows or rows that do not start on 16-byte boundaries: a row in registers
+//   norm_fwd_ring_kernel   forward, many rows: rows arrive in shared memory by bulk copies, several ahead
+//   norm_bwd_ring_kernel   backward: the same for x and dy, with the sums for dw and db in registers
+//   norm_bwd_kernel        backward without 16-byte boundaries: the next row is fetched into registers
+//   *_loop_kernel, norm_param_kernel   rows too long for the registers of 512 threads
 #include "common.cuh"
 #include "kernels.h"
+#include "tensor_core.cuh"
 
 namespace aq
 {
@@ -18,10 +23,10 @@ namespace
 {
 constexpr int kLoopThreads = 256;
 
-// Sum of two floats over the TPR threads of a row (a warp, or the whole CTA); every thread gets both.  `red` holds
-// 2 * 32 floats; consecutive calls of a CTA have to use different ones (one barrier each).
+// Sum of two floats over the TPR threads of a row (a warp, or the whole CTA); every thread gets both.  Consecutive calls
+// of a CTA have to use different `red` (one barrier each).
 template <int TPR>
-__device__ __forceinline__ float2 row_sum2(float a, float b, float* red)
+__device__ __forceinline__ float2 row_sum2(float a, float b, float4 (&red)[8])
 {
 #pragma unroll
     for (int o = 16; o; o >>= 1)
@@ -32,19 +37,19 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float* red)
     if constexpr (TPR > 32)
     {
         constexpr int WARPS = TPR / 32;
-        const int warp      = threadIdx.x >> 5;
+        static_assert(WARPS <= 16 && WARPS % 2 == 0, "two warps per 16 bytes");
         if ((threadIdx.x & 31) == 0)
-        {
-            red[warp]      = a;
-            red[32 + warp] = b;
-        }
+            reinterpret_cast<float2*>(red)[threadIdx.x >> 5] = make_float2(a, b);
         __syncthreads();
         a = b = 0.f;
 #pragma unroll
-        for (int i = 0; i < WARPS; ++i)
+        for (int i = 0; i < WARPS / 2; ++i)
         {
-            a += red[i];
-            b += red[32 + i];
+            const float4 r = red[i];
+            a += r.x;
+            b += r.y;
+            a += r.z;
+            b += r.w;
         }
     }
     return make_float2(a, b);
@@ -60,61 +65,125 @@ __device__ __forceinline__ Pack<T, VEC> splat(float v)
     return p;
 }
 
-// ------------------------------------------------------------------------------------------------------------------
-// Forward, row in registers: TPR threads hold PACKS packets of VEC elements each, packet k of thread t at (k TPR + t) VEC.
-// TPR = 32: four rows per CTA, one per warp.  w and b come out of L1 for every row.
-// ------------------------------------------------------------------------------------------------------------------
-template <typename T, int VEC, int TPR, int PACKS>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(LayerNormArgs a)
+// Elements 2q and 2q + 1 of a thread's packets as two float32 lanes (the last lane of an odd count is 0).
+template <typename T, int VEC, int PACKS>
+__device__ __forceinline__ f32x2_t lanes(const Pack<T, VEC> (&p)[PACKS], int q)
 {
-    constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
-    __shared__ float red[2][64];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int t       = threadIdx.x % TPR;
-    const int64_t row = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR;
-    if (ROWS > 1 && row >= a.rows)
-        return;   // whole warps, and no barrier follows
-    const T* x = (const T*) a.x + row * a.ldx;
-    Pack<T, VEC> v[PACKS];
-#pragma unroll
-    for (int k = 0; k < PACKS; ++k)
+    const int i = 2 * q, j = 2 * q + 1;
+    return pair(to_f32(p[i / VEC].v[i % VEC]), j < PACKS * VEC ? to_f32(p[j / VEC].v[j % VEC]) : 0.f);
+}
+template <typename T, int VEC, int PACKS>
+__device__ __forceinline__ void set_lanes(Pack<T, VEC> (&p)[PACKS], int q, f32x2_t v)
+{
+    float lo, hi;
+    unpair(v, lo, hi);
+    const int i = 2 * q, j = 2 * q + 1;
+    p[i / VEC].v[i % VEC] = from_f32<T>(lo);
+    if (j < PACKS * VEC)
+        p[j / VEC].v[j % VEC] = from_f32<T>(hi);
+}
+__device__ __forceinline__ float lane_sum(f32x2_t v)
+{
+    float lo, hi;
+    unpair(v, lo, hi);
+    return lo + hi;
+}
+
+// A packet, or `fill` in every element.  Through whole registers: element-wise selects would make the compiler wait for
+// each load before it issues the next.
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_or(const T* p, bool in, float fill)
+{
+    Pack<T, VEC> r = splat<T, VEC>(fill);
+    if constexpr (sizeof(r) == 16)
     {
-        const int64_t i = ((int64_t) k * TPR + t) * VEC;
-        v[k]            = i < a.dim ? load_pack<T, VEC>(x + i) : splat<T, VEC>(0.f);
+        uint4 u;
+        memcpy(&u, &r, 16);
+        if (in)
+            u = *reinterpret_cast<const uint4*>(p);
+        memcpy(&r, &u, 16);
     }
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < PACKS; ++k)
-#pragma unroll
-        for (int c = 0; c < VEC; ++c)
-            s += to_f32(v[k].v[c]);
-    const float mu = row_sum2<TPR>(s, 0.f, red[0]).x / (float) a.dim;
-    s              = 0.f;
-#pragma unroll
-    for (int k = 0; k < PACKS; ++k)
-        if (((int64_t) k * TPR + t) * VEC < a.dim)
-#pragma unroll
-            for (int c = 0; c < VEC; ++c)
-            {
-                const float d = to_f32(v[k].v[c]) - mu;
-                s             = fmaf(d, d, s);
-            }
-    const float rstd = 1.f / sqrtf(row_sum2<TPR>(s, 0.f, red[1]).x / (float) a.dim + a.eps);
-    T* y             = (T*) a.y + row * a.dim;
+    else if (in)
+        r = load_pack<T, VEC>(p);
+    return r;
+}
+
+// A thread's packets of one row: packet k of thread t starts at element (k TPR + t) VEC; what lies beyond the row is `fill`.
+template <typename T, int VEC, int TPR, int PACKS>
+__device__ __forceinline__ void load_row(Pack<T, VEC> (&p)[PACKS], const T* row, int t, int64_t dim, float fill)
+{
 #pragma unroll
     for (int k = 0; k < PACKS; ++k)
     {
         const int64_t i = ((int64_t) k * TPR + t) * VEC;
-        if (i < a.dim)
-        {
-            const Pack<T, VEC> w = a.w ? load_pack<T, VEC>((const T*) a.w + i) : splat<T, VEC>(1.f);
-            const Pack<T, VEC> b = a.b ? load_pack<T, VEC>((const T*) a.b + i) : splat<T, VEC>(0.f);
-            Pack<T, VEC> o;
+        p[k]            = load_or<T, VEC>(row + i, row && i < dim, fill);
+    }
+}
+template <typename T, int VEC, int TPR, int PACKS>
+__device__ __forceinline__ void store_row(const Pack<T, VEC> (&p)[PACKS], T* row, int t, int64_t dim)
+{
 #pragma unroll
-            for (int c = 0; c < VEC; ++c)
-                o.v[c] = from_f32<T>(fmaf((to_f32(v[k].v[c]) - mu) * rstd, to_f32(w.v[c]), to_f32(b.v[c])));
-            store_pack<T, VEC>(y + i, o);
+    for (int k = 0; k < PACKS; ++k)
+    {
+        const int64_t i = ((int64_t) k * TPR + t) * VEC;
+        if (i < dim)
+            store_pack<T, VEC>(row + i, p[k]);
+    }
+}
+
+// Statistics and result of a row whose packets are in v; `after_read` runs once every thread of the row has v in registers.
+// w and b come out of L1.  The arithmetic runs two float32 lanes per instruction.
+template <typename T, int VEC, int TPR, int PACKS, typename F>
+__device__ __forceinline__ void norm_row(const LayerNormArgs& a, const Pack<T, VEC> (&v)[PACKS], int64_t row, int t,
+                                         float4 (&red)[2][8], F&& after_read)
+{
+    constexpr int Q = (PACKS * VEC + 1) / 2;
+    f32x2_t s2 = pair(0.f, 0.f);
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        s2 = add2(s2, lanes(v, q));
+    const float mu   = row_sum2<TPR>(lane_sum(s2), 0.f, red[0]).x / (float) a.dim;
+    after_read();
+    const f32x2_t m2 = pair(mu, mu);
+    s2               = pair(0.f, 0.f);
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+    {
+        f32x2_t d = sub2(lanes(v, q), m2);
+        // packets beyond the row hold zeros, not the mean: take them out again
+        float lo, hi;
+        unpair(d, lo, hi);
+        const int64_t i = ((int64_t) (2 * q / VEC) * TPR + t) * VEC, j = ((int64_t) ((2 * q + 1) / VEC) * TPR + t) * VEC;
+        d               = pair(i < a.dim ? lo : 0.f, j < a.dim && 2 * q + 1 < PACKS * VEC ? hi : 0.f);
+        s2              = fma2(d, d, s2);
+    }
+    const float rstd = 1.f / sqrtf(row_sum2<TPR>(lane_sum(s2), 0.f, red[1]).x / (float) a.dim + a.eps);
+    const f32x2_t r2 = pair(rstd, rstd);
+    // eight lanes' worth of w and b at a time, so that they need few registers beside the row
+    constexpr int AT = PACKS < 2 ? PACKS : 2;
+#pragma unroll
+    for (int k0 = 0; k0 < PACKS; k0 += AT)
+    {
+        Pack<T, VEC> w[AT], b[AT], o[AT];
+#pragma unroll
+        for (int k = 0; k < AT; ++k)
+        {
+            const int64_t i = ((int64_t) (k0 + k) * TPR + t) * VEC;
+            const bool in   = k0 + k < PACKS && i < a.dim;
+            w[k]            = load_or<T, VEC>((const T*) a.w + i, a.w && in, 1.f);
+            b[k]            = load_or<T, VEC>((const T*) a.b + i, a.b && in, 0.f);
+            if (k0 + k < PACKS)
+                o[k] = v[k0 + k];
+        }
+#pragma unroll
+        for (int q = 0; q < (AT * VEC + 1) / 2; ++q)
+            set_lanes(o, q, fma2(mul2(sub2(lanes(o, q), m2), r2), lanes(w, q), lanes(b, q)));
+#pragma unroll
+        for (int k = 0; k < AT; ++k)
+        {
+            const int64_t i = ((int64_t) (k0 + k) * TPR + t) * VEC;
+            if (k0 + k < PACKS && i < a.dim)
+                store_pack<T, VEC>((T*) a.y + row * a.dim + i, o[k]);
         }
     }
     if (t == 0 && a.mean)
@@ -125,139 +194,398 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(LayerNo
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Backward, row in registers.  A thread keeps the same columns for every row its CTA takes, so the sums for dw and db
-// stay in its registers; the next row is fetched while the current one is reduced.  Each CTA leaves one row of partial
-// sums, part [gridDim.x][2][dim] (TPR = 32: the warps of the CTA are added up in shared memory first).
+// Forward, row in registers.  TPR = 32: four rows per CTA, one per warp.
 // ------------------------------------------------------------------------------------------------------------------
 template <typename T, int VEC, int TPR, int PACKS>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_bwd_kernel(LayerNormGradArgs a)
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(LayerNormArgs a)
 {
-    constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
+    constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
+    __shared__ float4 red[2][8];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t       = threadIdx.x % TPR;
+    const int64_t row = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR;
+    if (ROWS > 1 && row >= a.rows)
+        return;   // whole warps, and no barrier follows
+    Pack<T, VEC> v[PACKS];
+    load_row<T, VEC, TPR>(v, (const T*) a.x + row * a.ldx, t, a.dim, 0.f);
+    norm_row<T, VEC, TPR>(a, v, row, t, red, [] {});
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Forward and backward with a ring of rows in shared memory.  One thread of a row's group (a warp, or the CTA) keeps
+// `stages` rows on their way with bulk copies, so that the memory system sees 100 to 200 KB in flight per SM however
+// long the reductions of a row take; with the next row in registers alone it was 16 KB, and the backward pass of 16384
+// x 4096 bf16 took 168 us.  The waits are bounded (see mbar_wait).
+// ------------------------------------------------------------------------------------------------------------------
+__device__ int g_stuck;
+
+template <int TPR>
+struct RingShape
+{
+    static constexpr int kThreads = TPR < 128 ? 256 : TPR;
+    static constexpr int kGroups  = TPR < 128 ? 256 / TPR : 1;
+    static_assert(kGroups == 1 || TPR == 32, "a row belongs to a warp or to the CTA");
+};
+
+// CTAs per SM that registers allow when a thread needs about `regs`
+constexpr int ctas_for(int regs, int threads)
+{
+    const int n = 65536 / ((regs + 7) / 8 * 8 * threads);
+    return n < 1 ? 1 : n > 8 ? 8 : n;
+}
+
+// dynamic shared memory: [group][stage][MATRICES][dim] of T, then the barriers [group][stage]
+template <typename T, int MATRICES>
+struct Ring
+{
+    uint32_t data, bars, row_bytes;
+    int stages, stage = 0;
+    uint32_t phase    = 0;
+    volatile int* stuck;
+
+    __device__ __forceinline__ Ring(uint32_t base, int groups, int group, int stages_, int64_t dim, volatile int* stuck_)
+        : row_bytes((uint32_t) dim * sizeof(T)), stages(stages_), stuck(stuck_)
+    {
+        data = base + group * stages * MATRICES * row_bytes;
+        bars = base + groups * stages * MATRICES * row_bytes + group * stages * 8;
+    }
+    __device__ __forceinline__ uint32_t at(int s, int matrix) const
+    {
+        return data + (s * MATRICES + matrix) * row_bytes;
+    }
+    __device__ __forceinline__ void request(int s, const T* p0, const T* p1 = nullptr)
+    {
+        const uint32_t bar = bars + 8 * s;
+        tc::mbar_expect(bar, MATRICES * row_bytes);
+        tc::bulk_load(at(s, 0), p0, row_bytes, bar);
+        if (MATRICES == 2)
+            tc::bulk_load(at(s, 1), p1, row_bytes, bar);
+    }
+    __device__ __forceinline__ bool wait()
+    {
+        return tc::mbar_wait(bars + 8 * stage, phase, stuck);
+    }
+    __device__ __forceinline__ void advance()
+    {
+        if (++stage == stages)
+        {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
+template <typename T, int VEC, int TPR, int PACKS>
+__device__ __forceinline__ void read_row(Pack<T, VEC> (&p)[PACKS], uint32_t row, int t, int64_t dim)
+{
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k)
+    {
+        const int i = (k * TPR + t) * VEC;
+        uint4 u     = make_uint4(0, 0, 0, 0);
+        if (i < dim)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                         : "r"(row + i * (uint32_t) sizeof(T))
+                         : "memory");
+        memcpy(&p[k], &u, 16);
+    }
+}
+
+template <typename T, int TPR, int PACKS>
+__global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(4 * PACKS + 44, RingShape<TPR>::kThreads))
+    norm_fwd_ring_kernel(LayerNormArgs a, int stages)
+{
+    constexpr int VEC = 16 / (int) sizeof(T), GROUPS = RingShape<TPR>::kGroups;
+    extern __shared__ __align__(128) uint8_t ring_smem[];
+    __shared__ float4 red[2][8];
+    __shared__ int stuck_smem;
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    Ring<T, 1> ring(tc::smem_addr(ring_smem), GROUPS, group, stages, a.dim, &stuck_smem);
+    pdl_launch_dependents();
+    if (threadIdx.x == 0)
+        stuck_smem = 0;
+    if (t < stages)
+        tc::mbar_init(ring.bars + 8 * t, 1);
+    tc::mbar_init_fence();
+    __syncthreads();
+    pdl_wait();
+    const int64_t stride = (int64_t) gridDim.x * GROUPS;
+    int64_t row          = (int64_t) blockIdx.x * GROUPS + group;
+    const T* x           = (const T*) a.x;
+    if (t == 0)
+        for (int s = 0; s < stages && row + s * stride < a.rows; ++s)
+            ring.request(s, x + (row + s * stride) * a.ldx);
+    for (; row < a.rows; row += stride)
+    {
+        const bool ok = ring.wait();
+        Pack<T, VEC> v[PACKS];
+        read_row<T, VEC, TPR>(v, ring.at(ring.stage, 0), t, a.dim);
+        if (!ok)
+            v[0] = splat<T, VEC>(__int_as_float(0x7fffffff));
+        if (TPR == 32)
+            __syncwarp();
+        const int s        = ring.stage;
+        const int64_t next = row + stages * stride;
+        norm_row<T, VEC, TPR>(a, v, row, t, red, [&] {
+            // the barrier inside the row's first sum (or the warp's) is behind every thread: the stage is free
+            if (t == 0 && next < a.rows)
+                ring.request(s, x + next * a.ldx);
+        });
+        ring.advance();
+    }
+    __syncthreads();
+    tc::stuck_exit(&stuck_smem, &g_stuck);
+}
+
+// A thread keeps the same columns for every row its group takes; their sums for dw and db stay in its registers.  h and
+// dy w are formed twice, once for the sums of the row and once for dx, from the packets in shared memory.  Each CTA
+// leaves one row of partial sums, part [gridDim.x][2][dim] (TPR = 32: its warps are added up in shared memory first).
+template <typename T, int TPR, int PACKS>
+__global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(2 * PACKS * (16 / (int) sizeof(T)) + 44, RingShape<TPR>::kThreads))
+    norm_bwd_ring_kernel(LayerNormGradArgs a, int stages)
+{
+    constexpr int VEC = 16 / (int) sizeof(T), GROUPS = RingShape<TPR>::kGroups;
+    constexpr int N = PACKS * VEC, Q = N / 2;
+    extern __shared__ __align__(128) uint8_t ring_smem[];
+    __shared__ float4 red[2][8];
+    __shared__ int stuck_smem;
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    Ring<T, 2> ring(tc::smem_addr(ring_smem), GROUPS, group, stages, a.dim, &stuck_smem);
+    pdl_launch_dependents();
+    if (threadIdx.x == 0)
+        stuck_smem = 0;
+    if (t < stages)
+        tc::mbar_init(ring.bars + 8 * t, 1);
+    tc::mbar_init_fence();
+    __syncthreads();
+    pdl_wait();
+    const int64_t stride = (int64_t) gridDim.x * GROUPS;
+    int64_t row          = (int64_t) blockIdx.x * GROUPS + group;
+    auto request         = [&](int s, int64_t r) {
+        ring.request(s, (const T*) a.x + r * a.ldx, (const T*) a.dy + r * a.lddy);
+    };
+    // a CTA's stage is requested again one row later than it is read, behind that row's barrier
+    const int ahead = GROUPS > 1 ? stages : stages - 1;
+    if (t == 0)
+        for (int s = 0; s < ahead && row + s * stride < a.rows; ++s)
+            request(s, row + s * stride);
+    const f32x2_t zero = pair(0.f, 0.f);
+    f32x2_t dw[Q], db[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        dw[q] = db[q] = zero;
+    Pack<T, VEC> w[PACKS];
+    load_row<T, VEC, TPR>(w, (const T*) a.w, t, a.dim, 1.f);
+    float mu = 0.f, rstd = 0.f;
+    if (row < a.rows)
+    {
+        mu   = a.mean[row];
+        rstd = a.rstd[row];
+    }
+    for (int slot = 0; row < a.rows; row += stride, slot ^= 1)
+    {
+        const float r    = rstd;
+        const f32x2_t m2 = pair(mu, mu), r2 = pair(r, r);
+        if (row + stride < a.rows)
+        {
+            mu   = a.mean[row + stride];
+            rstd = a.rstd[row + stride];
+        }
+        const bool ok = ring.wait();
+        const uint32_t at_x = ring.at(ring.stage, 0), at_g = ring.at(ring.stage, 1);
+        f32x2_t sg = zero, sgh = zero;
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k)
+        {
+            Pack<T, VEC> x[1], g[1], wk[1] = {w[k]};
+            read_row<T, VEC, TPR>(x, at_x + k * TPR * 16, t, a.dim - k * TPR * VEC);
+            read_row<T, VEC, TPR>(g, at_g + k * TPR * 16, t, a.dim - k * TPR * VEC);
+#pragma unroll
+            for (int q = 0; q < VEC / 2; ++q)
+            {
+                const int i      = k * (VEC / 2) + q;
+                const f32x2_t dy = lanes(g, q);
+                const f32x2_t h  = mul2(sub2(lanes(x, q), m2), r2);
+                const f32x2_t gw = mul2(dy, lanes(wk, q));
+                dw[i]            = fma2(dy, h, dw[i]);
+                db[i]            = add2(db[i], dy);
+                sg               = add2(sg, gw);
+                sgh              = fma2(gw, h, sgh);
+            }
+        }
+        float2 sum = row_sum2<TPR>(lane_sum(sg), lane_sum(sgh), red[slot]);
+        if (!ok)
+            sum.x = __int_as_float(0x7fffffff);
+        if (GROUPS == 1 && t == 0 && row + ahead * stride < a.rows)
+            request(ring.stage == 0 ? stages - 1 : ring.stage - 1, row + ahead * stride);
+        if (a.dx)
+        {
+            // dx = r gw - r mean(g) - h r mean(g h)
+            const float c0 = -r * (sum.x / (float) a.dim), c1 = -r * (sum.y / (float) a.dim);
+            const f32x2_t c02 = pair(c0, c0), c12 = pair(c1, c1);
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k)
+            {
+                const int64_t i = ((int64_t) k * TPR + t) * VEC;
+                if (i >= a.dim)
+                    continue;
+                Pack<T, VEC> x[1], g[1], o[1], wk[1] = {w[k]};
+                read_row<T, VEC, TPR>(x, at_x + k * TPR * 16, t, a.dim - k * TPR * VEC);
+                read_row<T, VEC, TPR>(g, at_g + k * TPR * 16, t, a.dim - k * TPR * VEC);
+#pragma unroll
+                for (int q = 0; q < VEC / 2; ++q)
+                    set_lanes(o, q, fma2(mul2(sub2(lanes(x, q), m2), r2), c12, fma2(mul2(lanes(g, q), lanes(wk, q)), r2, c02)));
+                store_pack<T, VEC>((T*) a.dx + row * a.dim + i, o[0]);
+            }
+        }
+        if (GROUPS > 1)
+        {
+            __syncwarp();
+            if (t == 0 && row + ahead * stride < a.rows)
+                request(ring.stage, row + ahead * stride);
+        }
+        ring.advance();
+    }
+    __syncthreads();
+    tc::stuck_exit(&stuck_smem, &g_stuck);
+    if (!a.part)
+        return;
+    float* part = a.part + (int64_t) blockIdx.x * 2 * a.dim;
+    float* sums = reinterpret_cast<float*>(ring_smem);   // [GROUPS][dim]: the ring is no longer needed
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+    {
+        Pack<float, VEC> o[PACKS];
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            set_lanes(o, q, which ? db[q] : dw[q]);
+        if constexpr (GROUPS == 1)
+            store_row<float, VEC, TPR>(o, part + which * a.dim, t, a.dim);
+        else
+        {
+            __syncthreads();
+            store_row<float, VEC, TPR>(o, sums + group * a.dim, t, a.dim);
+            __syncthreads();
+            for (int i = threadIdx.x; i < a.dim; i += 256)
+            {
+                float s = 0.f;
+#pragma unroll
+                for (int j = 0; j < GROUPS; ++j)
+                    s += sums[j * a.dim + i];
+                part[which * a.dim + i] = s;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Backward without 16-byte boundaries: as norm_bwd_ring_kernel, but the next row is fetched into registers while the
+// current one is reduced.
+// ------------------------------------------------------------------------------------------------------------------
+template <int TPR, int COLUMNS>
+struct BwdShape
+{
+    static constexpr int kThreads = TPR < 128 ? 256 : TPR;
+    static constexpr int kRows    = TPR < 128 ? 256 / TPR : 1;
+    // resident CTAs per SM that the registers allow: about 5 per column and 32 more
+    static constexpr int kCtas = 65536 / ((5 * COLUMNS + 40) * kThreads) < 1 ? 1 : 65536 / ((5 * COLUMNS + 40) * kThreads);
+};
+
+template <typename T, int VEC, int TPR, int PACKS>
+__global__ void __launch_bounds__(BwdShape<TPR, PACKS * VEC>::kThreads, BwdShape<TPR, PACKS * VEC>::kCtas)
+    norm_bwd_kernel(LayerNormGradArgs a)
+{
+    constexpr int ROWS = BwdShape<TPR, PACKS * VEC>::kRows;
+    constexpr int N = PACKS * VEC, Q = (N + 1) / 2;
+    constexpr bool AHEAD = N <= 16;   // with more columns the registers of 512 threads do not hold the next row
     static_assert(ROWS == 1 || TPR == 32, "a row belongs to a warp or to the CTA");
-    __shared__ float red[2][64];
-    __shared__ float sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? TPR * PACKS * VEC + 1 : 1];
+    __shared__ float4 red[2][8];
+    __shared__ float sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? TPR * N + 1 : 1];
     pdl_launch_dependents();
     pdl_wait();
     const int t          = threadIdx.x % TPR;
     const int64_t stride = (int64_t) gridDim.x * ROWS;
-    const T* w           = (const T*) a.w;
-    const bool params    = a.part != nullptr;
-    float dw[PACKS][VEC], db[PACKS][VEC];
+    const f32x2_t zero   = pair(0.f, 0.f);
+    f32x2_t dw[Q], db[Q];
 #pragma unroll
-    for (int k = 0; k < PACKS; ++k)
-#pragma unroll
-        for (int c = 0; c < VEC; ++c)
-            dw[k][c] = db[k][c] = 0.f;
+    for (int q = 0; q < Q; ++q)
+        dw[q] = db[q] = zero;
     Pack<T, VEC> x[PACKS], g[PACKS];
     float mu = 0.f, rstd = 0.f;
     auto fetch = [&](int64_t row) {
         mu   = a.mean[row];
         rstd = a.rstd[row];
-#pragma unroll
-        for (int k = 0; k < PACKS; ++k)
-        {
-            const int64_t i = ((int64_t) k * TPR + t) * VEC;
-            if (i < a.dim)
-            {
-                x[k] = load_pack<T, VEC>((const T*) a.x + row * a.ldx + i);
-                g[k] = load_pack<T, VEC>((const T*) a.dy + row * a.lddy + i);
-            }
-            else
-            {
-                x[k] = splat<T, VEC>(0.f);
-                g[k] = splat<T, VEC>(0.f);
-            }
-        }
+        load_row<T, VEC, TPR>(x, (const T*) a.x + row * a.ldx, t, a.dim, 0.f);
+        load_row<T, VEC, TPR>(g, (const T*) a.dy + row * a.lddy, t, a.dim, 0.f);   // no part in any sum beyond the row
     };
     int64_t row = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR;
-    if (row < a.rows)
+    if (AHEAD && row < a.rows)
         fetch(row);
     for (int slot = 0; row < a.rows; row += stride, slot ^= 1)
     {
-        const float m = mu, r = rstd;
-        float sg = 0.f, sgh = 0.f;
-        Pack<T, VEC> cx[PACKS], cg[PACKS];
+        if (!AHEAD)
+            fetch(row);
+        const float r = rstd;
+        const f32x2_t m2 = pair(mu, mu), r2 = pair(r, r);
+        f32x2_t h[Q], gw[Q], sg = zero, sgh = zero;
+        Pack<T, VEC> w[PACKS];
+        load_row<T, VEC, TPR>(w, (const T*) a.w, t, a.dim, 1.f);
 #pragma unroll
-        for (int k = 0; k < PACKS; ++k)
+        for (int q = 0; q < Q; ++q)
         {
-            cx[k] = x[k];
-            cg[k] = g[k];
+            const f32x2_t dy = lanes(g, q);
+            const f32x2_t hq = mul2(sub2(lanes(x, q), m2), r2);
+            const f32x2_t gq = mul2(dy, lanes(w, q));
+            dw[q]            = fma2(dy, hq, dw[q]);
+            db[q]            = add2(db[q], dy);
+            sg               = add2(sg, gq);
+            sgh              = fma2(gq, hq, sgh);
+            h[q]             = hq;
+            gw[q]            = gq;
         }
-        if (row + stride < a.rows)
+        if (AHEAD && row + stride < a.rows)
             fetch(row + stride);
-#pragma unroll
-        for (int k = 0; k < PACKS; ++k)
-        {
-            const int64_t i = ((int64_t) k * TPR + t) * VEC;
-            if (i >= a.dim)
-                continue;
-            const Pack<T, VEC> wk = w ? load_pack<T, VEC>(w + i) : splat<T, VEC>(1.f);
-#pragma unroll
-            for (int c = 0; c < VEC; ++c)
-            {
-                const float dy = to_f32(cg[k].v[c]);
-                const float h  = (to_f32(cx[k].v[c]) - m) * r;
-                const float gw = dy * to_f32(wk.v[c]);
-                dw[k][c]       = fmaf(dy, h, dw[k][c]);
-                db[k][c] += dy;
-                sg += gw;
-                sgh = fmaf(gw, h, sgh);
-            }
-        }
         if (!a.dx)
             continue;
-        const float2 s  = row_sum2<TPR>(sg, sgh, red[slot]);
-        const float mg  = s.x / (float) a.dim;
-        const float mgh = s.y / (float) a.dim;
-        T* dx           = (T*) a.dx + row * a.dim;
+        const float2 s = row_sum2<TPR>(lane_sum(sg), lane_sum(sgh), red[slot]);
+        // dx = r gw - r mean(g) - h r mean(g h)
+        const float c0 = -r * (s.x / (float) a.dim), c1 = -r * (s.y / (float) a.dim);
+        const f32x2_t c02 = pair(c0, c0), c12 = pair(c1, c1);
+        Pack<T, VEC> o[PACKS];
 #pragma unroll
-        for (int k = 0; k < PACKS; ++k)
-        {
-            const int64_t i = ((int64_t) k * TPR + t) * VEC;
-            if (i >= a.dim)
-                continue;
-            const Pack<T, VEC> wk = w ? load_pack<T, VEC>(w + i) : splat<T, VEC>(1.f);
-            Pack<T, VEC> o;
-#pragma unroll
-            for (int c = 0; c < VEC; ++c)
-            {
-                const float h = (to_f32(cx[k].v[c]) - m) * r;
-                o.v[c]        = from_f32<T>(r * (to_f32(cg[k].v[c]) * to_f32(wk.v[c]) - mg - h * mgh));
-            }
-            store_pack<T, VEC>(dx + i, o);
-        }
+        for (int q = 0; q < Q; ++q)
+            set_lanes(o, q, fma2(h[q], c12, fma2(gw[q], r2, c02)));
+        store_row<T, VEC, TPR>(o, (T*) a.dx + row * a.dim, t, a.dim);
     }
-    if (!params)
+    if (!a.part)
         return;
     float* part = a.part + (int64_t) blockIdx.x * 2 * a.dim;
-    if constexpr (ROWS == 1)
-    {
 #pragma unroll
-        for (int k = 0; k < PACKS; ++k)
+    for (int which = 0; which < 2; ++which)
+    {
+        if constexpr (ROWS == 1)
         {
-            const int64_t i = ((int64_t) k * TPR + t) * VEC;
-            if (i >= a.dim)
-                continue;
+            Pack<float, VEC> o[PACKS];
 #pragma unroll
-            for (int c = 0; c < VEC; ++c)
-            {
-                part[i + c]         = dw[k][c];
-                part[a.dim + i + c] = db[k][c];
-            }
+            for (int q = 0; q < Q; ++q)
+                set_lanes(o, q, which ? db[q] : dw[q]);
+            store_row<float, VEC, TPR>(o, part + which * a.dim, t, a.dim);
         }
-    }
-    else
-    {
-        const int warp = threadIdx.x / TPR;
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
+        else
         {
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < PACKS; ++k)
-#pragma unroll
-                for (int c = 0; c < VEC; ++c)
-                    sums[warp][(k * TPR + t) * VEC + c] = which ? db[k][c] : dw[k][c];
+            for (int q = 0; q < Q; ++q)
+            {
+                float lo, hi;
+                unpair(which ? db[q] : dw[q], lo, hi);
+                const int i = 2 * q, j = 2 * q + 1;
+                sums[threadIdx.x / TPR][((i / VEC) * TPR + t) * VEC + i % VEC] = lo;
+                if (j < N)
+                    sums[threadIdx.x / TPR][((j / VEC) * TPR + t) * VEC + j % VEC] = hi;
+            }
             __syncthreads();
             for (int i = threadIdx.x; i < a.dim; i += 256)
             {
@@ -277,7 +605,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_bwd_kernel(LayerNo
 template <typename T>
 __global__ void __launch_bounds__(kLoopThreads) norm_fwd_loop_kernel(LayerNormArgs a)
 {
-    __shared__ float red[2][64];
+    __shared__ float4 red[2][8];
     pdl_launch_dependents();
     pdl_wait();
     const T* w = (const T*) a.w;
@@ -316,7 +644,7 @@ __global__ void __launch_bounds__(kLoopThreads) norm_fwd_loop_kernel(LayerNormAr
 template <typename T>
 __global__ void __launch_bounds__(kLoopThreads) norm_bwd_loop_kernel(LayerNormGradArgs a)
 {
-    __shared__ float red[2][64];
+    __shared__ float4 red[2][8];
     pdl_launch_dependents();
     pdl_wait();
     const T* w = (const T*) a.w;
@@ -387,24 +715,22 @@ __global__ void __launch_bounds__(256) norm_param_kernel(LayerNormGradArgs a, in
 // ------------------------------------------------------------------------------------------------------------------
 // dispatch
 // ------------------------------------------------------------------------------------------------------------------
-// f(TPR, PACKS) for the smallest shape that holds `packets` packets, AQ_ERR_TOO_LARGE (and no call) when none does.
+#define AQ_SHAPE(TPR, PACKS)                                                                                        \
+    if constexpr (PACKS <= MAX_PACKS)                                                                               \
+        if (packets <= (TPR) * (PACKS))                                                                             \
+            return f(std::integral_constant<int, TPR> {}, std::integral_constant<int, PACKS> {});
+
+// f(TPR, PACKS) for the first shape that holds `packets` packets, AQ_ERR_TOO_LARGE (and no call) when none does.
 // MAX_PACKS bounds the registers a thread gives to its columns.
 template <int MAX_PACKS, typename F>
 int with_row_shape(int64_t packets, F&& f)
 {
-    auto go = [&](auto tpr, auto packs) { return f(tpr, packs); };
-    using std::integral_constant;
-#define AQ_SHAPE(TPR, PACKS)                                                                       \
-    if constexpr (PACKS <= MAX_PACKS)                                                              \
-        if (packets <= (TPR) * (PACKS))                                                            \
-            return go(integral_constant<int, TPR> {}, integral_constant<int, PACKS> {});
     AQ_SHAPE(32, 1)
     AQ_SHAPE(32, 2)
-    AQ_SHAPE(32, 4)
+    AQ_SHAPE(128, 1)
     AQ_SHAPE(256, 1)
-    AQ_SHAPE(256, 2)
-    AQ_SHAPE(256, 3)
-    AQ_SHAPE(256, 4)
+    AQ_SHAPE(512, 1)
+    AQ_SHAPE(512, 2)
     AQ_SHAPE(512, 3)
     AQ_SHAPE(512, 4)
     AQ_SHAPE(512, 6)
@@ -412,8 +738,47 @@ int with_row_shape(int64_t packets, F&& f)
     AQ_SHAPE(512, 12)
     AQ_SHAPE(512, 16)
     AQ_SHAPE(512, 24)
-#undef AQ_SHAPE
     return AQ_ERR_TOO_LARGE;
+}
+// the same for the forward ring, which keeps no sums: fewer threads and more packets per row
+template <int MAX_PACKS, typename F>
+int with_ring_shape(int64_t packets, F&& f)
+{
+    AQ_SHAPE(32, 1)
+    AQ_SHAPE(32, 2)
+    AQ_SHAPE(32, 4)
+    AQ_SHAPE(128, 2)
+    AQ_SHAPE(128, 4)
+    AQ_SHAPE(256, 4)
+    AQ_SHAPE(512, 4)
+    AQ_SHAPE(512, 8)
+    return AQ_ERR_TOO_LARGE;
+}
+#undef AQ_SHAPE
+
+// Stages of a ring: as many as fit with `ctas` CTAs on an SM (or fewer CTAs), 2 to 6; 0 when two do not fit.
+int ring_stages(int64_t stage_bytes, int groups, int& ctas)
+{
+    constexpr int64_t kBudget = 208 * 1024;
+    for (; ctas >= 1; --ctas)
+    {
+        const int64_t n = kBudget / ctas / (stage_bytes * groups + 8 * groups);
+        if (n >= (ctas > 1 ? 3 : 2))
+            return (int) (n < 6 ? n : 6);
+    }
+    return 0;
+}
+
+template <typename Args, typename Kernel>
+int launch_ring(Kernel kernel, const Args& a, int stages, int groups, int matrices, int64_t elem, int64_t grid, int threads,
+                cudaStream_t st)
+{
+    const int64_t smem = (int64_t) groups * stages * (matrices * a.dim * elem + 8);
+    cudaError_t e      = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
+    if (e == cudaSuccess)
+        e = launch_pdl(kernel, dim3((unsigned) grid), threads, (size_t) smem, st, a, stages);
+    note_launch();
+    return e == cudaSuccess ? AQ_OK : cuda_fail(e);
 }
 
 template <typename T>
@@ -428,9 +793,26 @@ bool wide_rows(const void* a, int64_t lda, const void* b, int64_t ldb, const voi
 template <typename T, int VEC>
 int norm_fwd_v(const LayerNormArgs& a, cudaStream_t st)
 {
-    return with_row_shape<VEC == 1 ? 24 : 8>((a.dim + VEC - 1) / VEC, [&](auto tpr, auto packs) {
-        constexpr int TPR = decltype(tpr)::value;
-        constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
+    const int64_t packets = (a.dim + VEC - 1) / VEC;
+    if constexpr (VEC > 1)
+    {
+        // the ring pays once its groups take several rows each; before that the plain form starts sooner
+        const int rc = with_ring_shape<8>(packets, [&](auto tpr, auto packs) -> int {
+            constexpr int TPR = decltype(tpr)::value, PACKS = decltype(packs)::value;
+            using S        = RingShape<TPR>;
+            int ctas       = ctas_for(4 * PACKS + 44, S::kThreads);
+            const int n    = ring_stages(a.dim * (int64_t) sizeof(T), S::kGroups, ctas);
+            const int64_t grid = (int64_t) ctas * kNumSMs;
+            if (n == 0 || a.rows < 2 * grid * S::kGroups)
+                return AQ_ERR_TOO_LARGE;
+            return launch_ring(norm_fwd_ring_kernel<T, TPR, PACKS>, a, n, S::kGroups, 1, sizeof(T), grid, S::kThreads, st);
+        });
+        if (rc != AQ_ERR_TOO_LARGE)
+            return rc;
+    }
+    return with_row_shape<VEC == 1 ? 24 : 8>(packets, [&](auto tpr, auto packs) {
+        constexpr int TPR   = decltype(tpr)::value;
+        constexpr int ROWS  = TPR < 128 ? 128 / TPR : 1;
         const cudaError_t e = launch_pdl(norm_fwd_kernel<T, VEC, TPR, decltype(packs)::value>,
                                          dim3((unsigned) ((a.rows + ROWS - 1) / ROWS)), TPR < 128 ? 128 : TPR, 0, st, a);
         note_launch();
@@ -451,20 +833,45 @@ int norm_fwd_t(const LayerNormArgs& a, cudaStream_t st)
     return e == cudaSuccess ? AQ_OK : cuda_fail(e);
 }
 
-constexpr int kBwdCtasPerSm = 2;
+// Most CTAs of the backward kernels, each with one row of partial sums: what the registers let reside anyway.
+int64_t bwd_ctas(int64_t rows, int64_t dim)
+{
+    const int64_t n = kNumSMs * (dim <= 1024 ? 8 : dim <= 2048 ? 4 : dim <= 4096 ? 2 : 1);
+    return rows < 1 ? 1 : rows < n ? rows : n;
+}
 
-template <typename T, int VEC>
-int norm_bwd_v(const LayerNormGradArgs& a, cudaStream_t st)
+template <typename T>
+int norm_bwd_wide(const LayerNormGradArgs& a, cudaStream_t st)
+{
+    constexpr int VEC = 16 / (int) sizeof(T);
+    // at most 32 columns per thread (64 running sums)
+    return with_row_shape<32 / VEC>(a.dim / VEC, [&](auto tpr, auto packs) -> int {
+        constexpr int TPR = decltype(tpr)::value, PACKS = decltype(packs)::value;
+        using S     = RingShape<TPR>;
+        int ctas    = ctas_for(2 * PACKS * VEC + 44, S::kThreads);
+        const int n = ring_stages(2 * a.dim * (int64_t) sizeof(T), S::kGroups, ctas);
+        if (n == 0)
+            return AQ_ERR_TOO_LARGE;
+        const int64_t most = bwd_ctas((a.rows + S::kGroups - 1) / S::kGroups, a.dim);
+        const int64_t grid = most < (int64_t) ctas * kNumSMs ? most : (int64_t) ctas * kNumSMs;
+        const int rc = launch_ring(norm_bwd_ring_kernel<T, TPR, PACKS>, a, n, S::kGroups, 2, sizeof(T), grid, S::kThreads, st);
+        if (rc != AQ_OK || !a.part)
+            return rc;
+        return fold_columns(a.part, grid, 2 * a.dim, a.dim, a.dw, a.db, a.dtype, st);
+    });
+}
+
+template <typename T>
+int norm_bwd_odd(const LayerNormGradArgs& a, cudaStream_t st)
 {
     // at most 24 columns per thread (48 running sums)
-    return with_row_shape<24 / VEC>((a.dim + VEC - 1) / VEC, [&](auto tpr, auto packs) {
-        constexpr int TPR  = decltype(tpr)::value;
-        constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
-        const int64_t most = (a.rows + ROWS - 1) / ROWS;
-        int64_t grid       = most < kBwdCtasPerSm * kNumSMs ? most : kBwdCtasPerSm * kNumSMs;
-        grid               = grid < 1 ? 1 : grid;
-        cudaError_t e = launch_pdl(norm_bwd_kernel<T, VEC, TPR, decltype(packs)::value>, dim3((unsigned) grid),
-                                   TPR < 256 ? 256 : TPR, 0, st, a);
+    return with_row_shape<24>(a.dim, [&](auto tpr, auto packs) {
+        using S            = BwdShape<decltype(tpr)::value, decltype(packs)::value>;
+        const int64_t most = bwd_ctas((a.rows + S::kRows - 1) / S::kRows, a.dim);
+        int64_t grid       = (S::kCtas < 4 ? S::kCtas : 4) * kNumSMs;
+        grid               = most < grid ? most : grid;
+        cudaError_t e      = launch_pdl(norm_bwd_kernel<T, 1, decltype(tpr)::value, decltype(packs)::value>,
+                                        dim3((unsigned) grid), S::kThreads, 0, st, a);
         note_launch();
         if (e != cudaSuccess)
             return cuda_fail(e);
@@ -486,7 +893,7 @@ template <typename T>
 int norm_bwd_t(const LayerNormGradArgs& a, cudaStream_t st)
 {
     const bool wide = wide_rows<T>(a.x, a.ldx, a.dy, a.lddy, a.w, nullptr, a.dx, a.dim);
-    const int rc    = wide ? norm_bwd_v<T, 16 / (int) sizeof(T)>(a, st) : norm_bwd_v<T, 1>(a, st);
+    const int rc    = wide ? norm_bwd_wide<T>(a, st) : norm_bwd_odd<T>(a, st);
     if (rc != AQ_ERR_TOO_LARGE)
         return rc;
     if (a.dx)
@@ -512,11 +919,15 @@ int norm_bwd_t(const LayerNormGradArgs& a, cudaStream_t st)
 
 int64_t norm_bwd_workspace_bytes(int64_t rows, int64_t dim)
 {
-    // one row of sums per CTA of norm_bwd_kernel or per band of norm_param_kernel
-    int64_t n           = rows < kBwdCtasPerSm * kNumSMs ? rows : kBwdCtasPerSm * kNumSMs;
-    const int64_t bands = norm_bands(rows, dim);
-    n                   = n < bands ? bands : n;
-    return (n < 1 ? 1 : n) * 2 * dim * (int64_t) sizeof(float);
+    // one row of sums per CTA of the register kernels or per band of norm_param_kernel
+    const int64_t ctas = bwd_ctas(rows, dim), bands = norm_bands(rows, dim);
+    return (ctas < bands ? bands : ctas) * 2 * dim * (int64_t) sizeof(float);
+}
+
+int norm_stuck(int* out)
+{
+    const cudaError_t e = cudaMemcpyFromSymbol(out, g_stuck, sizeof(int));
+    return e == cudaSuccess ? AQ_OK : cuda_fail(e);
 }
 
 int norm_fwd(const LayerNormArgs& a, cudaStream_t st)

@@ -224,10 +224,10 @@ int grad_z_t(const GradZArgs& a, cudaStream_t st)
 // Sums over the bands: out0[c] = sum_b part[b * stride + c], out1[c] the same at column cols + c.
 // ------------------------------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) fold_columns_kernel(const float* part, int64_t bands, int64_t stride, int64_t cols,
-                                                           T* out0, T* out1)
+__global__ void __launch_bounds__(1024) fold_columns_kernel(const float* part, int64_t bands, int64_t stride, int64_t cols,
+                                                            T* out0, T* out1)
 {
-    __shared__ float sh[8][32];
+    __shared__ float sh[32][32];
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -235,7 +235,8 @@ __global__ void __launch_bounds__(256) fold_columns_kernel(const float* part, in
     T* out            = blockIdx.y ? out1 : out0;
     float s           = 0.f;
     if (out && col < cols)
-        for (int64_t b = warp; b < bands; b += 8)
+#pragma unroll 4
+        for (int64_t b = warp; b < bands; b += 32)
             s += part[b * stride + (int64_t) blockIdx.y * cols + col];
     sh[warp][lane] = s;
     __syncthreads();
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(256) fold_columns_kernel(const float* part, in
     {
         s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 32; ++i)
             s += sh[i][lane];
         out[col] = from_f32<T>(s);
     }
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(256) fold_columns_kernel(const float* part, in
 template <typename T>
 int fold_columns_t(const float* part, int64_t bands, int64_t stride, int64_t cols, void* out0, void* out1, cudaStream_t st)
 {
-    const cudaError_t e = launch_pdl(fold_columns_kernel<T>, dim3((unsigned) ((cols + 31) / 32), out1 ? 2 : 1), 256, 0, st,
+    const cudaError_t e = launch_pdl(fold_columns_kernel<T>, dim3((unsigned) ((cols + 31) / 32), out1 ? 2 : 1), 1024, 0, st,
                                      part, bands, stride, cols, (T*) out0, (T*) out1);
     note_launch();
     return e == cudaSuccess ? AQ_OK : cuda_fail(e);

@@ -112,6 +112,14 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
+// `bytes` (a multiple of 16) from one 16-byte boundary to another
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 // ---- tensor memory ----------------------------------------------------------------------------------------------
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t cols)

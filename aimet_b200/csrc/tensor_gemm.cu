@@ -15,7 +15,7 @@ namespace
 {
 using namespace tc;
 
-__device__ int g_stuck;   // raised when a bounded wait ran out; read by aq_linear_stuck
+__device__ int g_stuck;   // raised when a bounded wait ran out; read by aq_layers_stuck
 
 struct TcArgs
 {
@@ -151,6 +151,37 @@ __device__ __forceinline__ void row_chunk(const TcArgs& p, const float* acc, int
             f[c] += to_f32(r[c]);
     }
     store_wide<T, N>((T*) p.out + i * p.ldo + j, f);
+}
+
+// One epilogue chunk of N rows (the first `most` of them exist) for a thread that holds one column of them; z is acc.
+// The residuals are fetched together: one at a time their latency is what the epilogue waits for (a 777 x 1537 result:
+// 30 us against 8 us).
+template <typename T, int N>
+__device__ __forceinline__ void column_chunk(const TcArgs& p, float (&acc)[N], int64_t i, int most, int64_t j)
+{
+    T r[N];
+    if (p.residual)
+    {
+        const T* src = (const T*) p.residual + i * p.ldr + j;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (u < most)
+                r[u] = src[u * p.ldr];
+    }
+    if (p.z)
+    {
+        T* dst = (T*) p.z + i * p.ldz + j;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (u < most)
+                dst[u * p.ldz] = from_f32<T>(acc[u]);
+    }
+    activate<N>(acc, p.act);
+    T* dst = (T*) p.out + i * p.ldo + j;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+        if (u < most)
+            dst[u * p.ldo] = from_f32<T>(p.residual ? acc[u] + to_f32(r[u]) : acc[u]);
 }
 
 template <typename T, int BN>
@@ -352,17 +383,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(128 + 32 * kPairWarp
                     {
                         const float bias = p.bias ? to_f32(((const T*) p.bias)[jj]) : 0.f;
                         const int most   = p.rows - row0 < 32 ? (int) (p.rows - row0) : 32;
-#pragma unroll 4
-                        for (int r = 0; r < most; ++r)
+#pragma unroll 1
+                        for (int r = 0; r < most; r += 16)
                         {
-                            const int64_t i = row0 + r;
-                            float v[1]      = {patch[r * 33 + lane] + bias};
-                            if (p.z)
-                                ((T*) p.z)[i * p.ldz + jj] = from_f32<T>(v[0]);
-                            activate<1>(v, p.act);
-                            if (p.residual)
-                                v[0] += to_f32(((const T*) p.residual)[i * p.ldr + jj]);
-                            ((T*) p.out)[i * p.ldo + jj] = from_f32<T>(v[0]);
+                            float v[16];
+#pragma unroll
+                            for (int u = 0; u < 16; ++u)
+                                v[u] = patch[(r + u) * 33 + lane] + bias;
+                            column_chunk<T, 16>(p, v, row0 + r, most - r, jj);
                         }
                     }
                 }
@@ -511,21 +539,12 @@ __global__ void __launch_bounds__(192, 2)
         poison = __any_sync(0xffffffffu, !mbar_wait(tfull, 0, stuck));
         tmem_fence_after();
     }
-    // one result of this thread's column
-    auto finish = [&](float acc, int64_t i) {
-        float v[1] = {(poison ? __int_as_float(0x7fffffff) : acc) + bias};
-        if (p.z)
-            ((T*) p.z)[i * p.ldz + j] = from_f32<T>(v[0]);
-        activate<1>(v, p.act);
-        if (p.residual)
-            v[0] += to_f32(((const T*) p.residual)[i * p.ldr + j]);
-        ((T*) p.out)[i * p.ldo + j] = from_f32<T>(v[0]);
-    };
+    const float bad = __int_as_float(0x7fffffff);
+    const int rows  = p.rows - i0 < BN ? (int) (p.rows - i0) : BN;
     if (warp >= 2)
     {
-        const int rows = p.rows - i0 < BN ? (int) (p.rows - i0) : BN;
 #pragma unroll 1
-        for (int c0 = 0; c0 < BN; c0 += 16)
+        for (int c0 = 0; c0 < rows; c0 += 16)
         {
             uint32_t raw[16];
             tmem_load16(tmem + c0 + ((uint32_t) (quarter * 32) << 16), raw);
@@ -534,14 +553,15 @@ __global__ void __launch_bounds__(192, 2)
             {
 #pragma unroll
                 for (int c = 0; c < 16; ++c)
-                    part[(c0 + c) * 128 + f] = poison ? __int_as_float(0x7fffffff) : __uint_as_float(raw[c]);
+                    part[(c0 + c) * 128 + f] = poison ? bad : __uint_as_float(raw[c]);
             }
             else if (j < p.cols)
             {
+                float v[16];
 #pragma unroll
                 for (int c = 0; c < 16; ++c)
-                    if (c0 + c < rows)
-                        finish(__uint_as_float(raw[c]), i0 + c0 + c);
+                    v[c] = (poison ? bad : __uint_as_float(raw[c])) + bias;
+                column_chunk<T, 16>(p, v, i0 + c0, rows - c0, j);
             }
         }
     }
@@ -551,15 +571,28 @@ __global__ void __launch_bounds__(192, 2)
         cluster_sync();
         if (warp >= 2 && j < p.cols)
         {
-            const int rows = p.rows - i0 < BN ? (int) (p.rows - i0) : BN;
             const int c0 = rows * (int) rank / (int) splits, c1 = rows * (int) (rank + 1) / (int) splits;
             const uint32_t mine = smem_addr(part) + f * 4;
-            for (int c = c0; c < c1; ++c)
+            constexpr int AT = BN < 8 * 8 ? 4 : 8;   // rows joined at a time
+#pragma unroll 1
+            for (int c = c0; c < c1; c += AT)
             {
-                float s = 0.f;
+                float v[AT] = {};
                 for (uint32_t r = 0; r < splits; ++r)   // always in this order: the same bits on every run
-                    s += ld_cluster(map_to(mine + c * 512, r));
-                finish(s, i0 + c);
+                {
+                    const uint32_t from = map_to(mine + c * 512, r);
+                    float w[AT];
+#pragma unroll
+                    for (int u = 0; u < AT; ++u)
+                        w[u] = c + u < c1 ? ld_cluster(from + u * 512) : 0.f;
+#pragma unroll
+                    for (int u = 0; u < AT; ++u)
+                        v[u] += w[u];
+                }
+#pragma unroll
+                for (int u = 0; u < AT; ++u)
+                    v[u] += bias;
+                column_chunk<T, AT>(p, v, i0 + c, c1 - c, j);
             }
         }
         __syncwarp();

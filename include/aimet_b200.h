@@ -544,9 +544,9 @@ int aq_linear_grad_input(const void* d_dz, int64_t lddz, const void* d_w, int64_
 int aq_linear_grad_weight(const void* d_dz, int64_t lddz, const void* d_x, int64_t ldx, void* d_dw, int64_t lddw,
                           int dtype, int64_t m, int64_t n, int64_t k, void* stream);
 
-/* Every wait inside the product kernels is bounded (4 s).  *h_out: 0, or 1 once a wait has run out on the current
- * device since the library was loaded; the tiles concerned hold NaN.  Copies from the device (synchronises). */
-int aq_linear_stuck(int* h_out);
+/* Every wait inside the layers' kernels is bounded (4 s).  *h_out: 0, or 1 once a wait has run out on the current
+ * device since the library was loaded; the results concerned hold NaN.  Copies from the device (synchronises). */
+int aq_layers_stuck(int* h_out);
 
 /* y = (x - mean) / sqrt(var + eps) * w + b over rows of dim elements (var: mean of squared differences).
  * d_w / d_b: dim elements of dtype, or NULL for 1 / 0.  d_mean, d_rstd: one float per row for the backward pass, both

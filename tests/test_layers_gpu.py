@@ -601,4 +601,4 @@ def test_no_wait_ran_out(cuda):
     import ctypes
     from aimet_b200._lib import lib
     out = ctypes.c_int(7)
-    assert lib.aq_linear_stuck(ctypes.byref(out)) == 0 and out.value == 0
+    assert lib.aq_layers_stuck(ctypes.byref(out)) == 0 and out.value == 0

@@ -49,13 +49,16 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     return m
 
 
-def _check_operand(t: Optional[torch.Tensor], like: torch.Tensor, name: str) -> None:
+def _check_operand(t: Optional[torch.Tensor], like: torch.Tensor, shape: tuple, name: str) -> None:
     if t is None:
         return
+    if t.shape != shape:
+        raise RuntimeError(f"aimet_b200: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     ops._cuda(t, name)   # pylint: disable=protected-access
-    ops._same_device(like, t)   # pylint: disable=protected-access
-    if t.dtype != like.dtype:
+    if t.dtype is not like.dtype:
         raise RuntimeError(f"aimet_b200: {name} is {t.dtype}, the input is {like.dtype}")
+    if t.get_device() != like.get_device():
+        ops._same_device(like, t)   # pylint: disable=protected-access
 
 
 def _wants_grad(*tensors) -> bool:
@@ -65,17 +68,22 @@ def _wants_grad(*tensors) -> bool:
 # ---------------------------------------------------------------------------------------------------
 # linear
 # ---------------------------------------------------------------------------------------------------
+def _new_rows(like: torch.Tensor, m: int, n: int) -> torch.Tensor:
+    """Uninitialised [m, n] whose rows the tensor cores can read."""
+    return like.new_empty((m, n)) if n % 8 == 0 else like.new_empty((m, (n + 7) // 8 * 8))[:, :n]
+
+
 def _linear_forward(x, weight, bias, residual, activation, keep_z):
-    n = weight.shape[0]
-    xm, wm = ops.aligned_rows(_rows(x, weight.shape[1])), ops.aligned_rows(_rows(weight, weight.shape[1]))
+    n, k = weight.shape
+    xm, wm = ops.aligned_rows(_rows(x, k)), ops.aligned_rows(_rows(weight, k))
     rm = None if residual is None else _rows(residual, n)
     bias = None if bias is None else bias.contiguous()
     m = xm.shape[0]
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    z = torch.empty((m, (n + 7) // 8 * 8), dtype=x.dtype, device=x.device)[:, :n] if keep_z else None
+    ym = x.new_empty((m, n))
+    z = _new_rows(x, m, n) if keep_z else None
     if m:
-        ops.linear_forward(xm, wm, bias, rm, activation, y.view(m, n), z)
-    return y, z, xm, wm
+        ops.linear_forward(xm, wm, bias, rm, activation, ym, z)
+    return ym if x.dim() == 2 else ym.view(x.shape[:-1] + (n,)), z, xm, wm
 
 
 class _LinearFn(torch.autograd.Function):
@@ -100,20 +108,22 @@ class _LinearFn(torch.autograd.Function):
         dy = _rows(_plain(grad), n)
         dx = dw = db = None
         if need_b:
-            db = torch.empty(n, dtype=dy.dtype, device=dy.device)
+            db = dy.new_empty(n)
         dz = dy
         if ctx.activation is not None and (need_x or need_w):
-            dz = torch.empty((m, (n + 7) // 8 * 8), dtype=dy.dtype, device=dy.device)[:, :n]
+            dz = _new_rows(dy, m, n)
         if need_b or dz is not dy:
             ops.linear_grad_z(dy, z, ctx.activation, None if dz is dy else dz, db)
         if need_x or need_w:
             dz = ops.aligned_rows(dz)
         if need_x:
-            dx = torch.empty(ctx.x_shape, dtype=dy.dtype, device=dy.device)
+            dx = dy.new_empty((m, k))
             if m:
-                ops.linear_grad_input(dz, wm, dx.view(m, k))
+                ops.linear_grad_input(dz, wm, dx)
+            if len(ctx.x_shape) != 2:
+                dx = dx.view(ctx.x_shape)
         if need_w:
-            dw = torch.empty((n, k), dtype=dy.dtype, device=dy.device)
+            dw = dy.new_empty((n, k))
             ops.linear_grad_weight(dz, xm, dw)
         return dx, dw, db, grad if need_r else None, None
 
@@ -137,14 +147,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         raise RuntimeError(f"aimet_b200: cannot apply a weight of shape {tuple(weight.shape)} to an input of shape "
                            f"{tuple(x.shape)}")
     n = weight.shape[0]
-    if bias is not None and tuple(bias.shape) != (n,):
-        raise RuntimeError(f"aimet_b200: bias must have shape ({n},), got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != x.shape[:-1] + (n,):
-        raise RuntimeError(f"aimet_b200: residual must have the result's shape {tuple(x.shape[:-1]) + (n,)}, got "
-                           f"{tuple(residual.shape)}")
-    _check_operand(weight, x, "weight")
-    _check_operand(bias, x, "bias")
-    _check_operand(residual, x, "residual")
+    _check_operand(weight, x, weight.shape, "weight")
+    _check_operand(bias, x, (n,), "bias")
+    _check_operand(residual, x, x.shape[:-1] + (n,), "residual")
     if _wants_grad(x, weight, bias, residual):
         return _LinearFn.apply(x, weight, bias, residual, activation)
     return _linear_forward(x, weight, bias, residual, activation, False)[0]
@@ -156,12 +161,15 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 def _norm_forward(x, dim, weight, bias, eps, keep_stats):
     xm = _rows(x, dim)
     rows = xm.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     w = None if weight is None else weight.contiguous()
     b = None if bias is None else bias.contiguous()
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep_stats else None
+    stats, mean, rstd = None, None, None
+    if keep_stats:
+        stats = x.new_empty((2, rows), dtype=torch.float32)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
     if rows:
-        mean, rstd = stats if keep_stats else (None, None)
         ops.layer_norm_forward(xm, w, b, eps, y, mean, rstd)
     return y, xm, w, stats
 
@@ -182,11 +190,11 @@ class _LayerNormFn(torch.autograd.Function):
         xm, w, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = _rows(_plain(grad), xm.shape[1])
-        new = lambda shape: torch.empty(shape, dtype=dy.dtype, device=dy.device)   # noqa: E731
-        dx = new(ctx.x_shape) if need_x else None
-        dw = new(ctx.w_shape) if need_w else None
-        db = new(ctx.w_shape) if need_b else None
-        ops.layer_norm_backward(xm, dy, w, stats[0], stats[1], dx, dw, db)
+        dx = dy.new_empty(ctx.x_shape) if need_x else None
+        dw = dy.new_empty(ctx.w_shape) if need_w else None
+        db = dy.new_empty(ctx.w_shape) if need_b else None
+        mean = stats.data_ptr()
+        ops.layer_norm_backward(xm, dy, w, mean, mean + 4 * xm.shape[0], dx, dw, db)
         return dx, dw, db, None, None
 
 
@@ -205,10 +213,8 @@ def layer_norm(x: torch.Tensor, normalized_shape: Union[int, Sequence[int]], wei
         raise RuntimeError(f"aimet_b200: cannot normalise an input of shape {tuple(x.shape)} over {shape}")
     if not 0 <= eps < math.inf:
         raise RuntimeError(f"aimet_b200: eps must be finite and at least 0, got {eps}")
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None and tuple(t.shape) != shape:
-            raise RuntimeError(f"aimet_b200: {name} must have shape {shape}, got {tuple(t.shape)}")
-        _check_operand(t, x, name)
+    _check_operand(weight, x, shape, "weight")
+    _check_operand(bias, x, shape, "bias")
     if _wants_grad(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, shape, eps)
     return _norm_forward(x, dim, weight, bias, eps, False)[0]

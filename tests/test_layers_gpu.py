@@ -523,7 +523,7 @@ def test_refusals_on_the_gpu(cuda):
     x, w = torch.randn(4, 16, device=cuda), torch.randn(8, 16, device=cuda)
     with pytest.raises(RuntimeError, match="weight is"):
         linear(x, w.half())
-    with pytest.raises(RuntimeError, match="residual must have"):
+    with pytest.raises(RuntimeError, match="residual must have shape"):
         linear(x, w, residual=torch.zeros(8, device=cuda))
     with pytest.raises(RuntimeError, match="bias must have shape"):
         linear(x, w, torch.zeros(4, device=cuda))

@@ -3,110 +3,207 @@
 #include "activation.cuh"
 #include "common.cuh"
 #include "kernels.h"
+#include "tensor_core.cuh"
 
 namespace aq
 {
 namespace
 {
 // ------------------------------------------------------------------------------------------------
-// out[i, j] = sum_k A[i, k] B[j, k] with float32 fused multiply-adds.  An operand is read as rows over k (KMAJOR:
-// element (i, k) at i * ld + k) or as columns (element (i, k) at k * ld + i).
+// float32 products: out[i, j] = sum_k A[i, k] B[j, k] with fused multiply-adds, two lanes per instruction.  (The tensor
+// cores would round the operands to 10 bits.)  An operand is read as rows over k (KMAJOR: element (i, k) at i * ld + k)
+// or as columns (element (i, k) at k * ld + i); either way a slice of 16 k lies in shared memory as [k][row].  The
+// copies are asynchronous and element-wise: they need no alignment, turn rows into columns on the way, and cost one
+// instruction per 32 fused multiply-adds.
+//
+// TILE x TILE results per CTA of 256 threads, TILE / 16 squared per thread; the depth can be split over a cluster, whose
+// CTAs then add up their partial tiles in a fixed order through distributed shared memory.
 // ------------------------------------------------------------------------------------------------
-constexpr int kTile = 64, kDepth = 16, kSimtThreads = 256;
+constexpr int kSimtThreads = 256, kDepth = 16;
 
-template <typename T, bool KMAJOR>
-__device__ __forceinline__ void simt_load(const T* p, int64_t ld, int64_t rows, int64_t k, int64_t row0, int64_t k0,
-                                          float (*dst)[kTile + 4])
+template <int TILE>
+struct SimtShape
+{
+    static constexpr int kPitch  = TILE + 4;   // [k][row]; the pad spreads the turned copies over the banks
+    static constexpr int kStages = 4;
+    static constexpr int kSlice  = kDepth * kPitch;                     // floats of one operand
+    static constexpr int kSmem   = kStages * 2 * kSlice * 4;
+    static_assert(TILE * TILE * 4 <= kSmem, "the partial tile takes the place of the operands");
+};
+
+__device__ __forceinline__ void copy_async4(uint32_t dst, const float* src, bool in)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+
+// Slice of TILE rows x 16 k from row0, k0; what lies outside the matrix becomes 0 (the address then is the matrix itself).
+template <int TILE, bool KMAJOR>
+__device__ __forceinline__ void simt_load(const float* p, int64_t ld, int64_t rows, int64_t k_end, int64_t row0, int64_t k0,
+                                          uint32_t dst)
 {
 #pragma unroll
-    for (int s = 0; s < kTile * kDepth / kSimtThreads; ++s)
+    for (int s = 0; s < TILE * kDepth / kSimtThreads; ++s)
     {
         const int e = s * kSimtThreads + threadIdx.x;
-        const int r = KMAJOR ? e / kDepth : e % kTile;
-        const int c = KMAJOR ? e % kDepth : e / kTile;
+        const int r = KMAJOR ? e / kDepth : e % TILE;
+        const int c = KMAJOR ? e % kDepth : e / TILE;
         const int64_t gr = row0 + r, gk = k0 + c;
-        float v = 0.f;
-        if (gr < rows && gk < k)
-            v = to_f32(p[KMAJOR ? gr * ld + gk : gk * ld + gr]);
-        dst[c][r] = v;
+        const bool in = gr < rows && gk < k_end;
+        copy_async4(dst + (c * SimtShape<TILE>::kPitch + r) * 4, in ? p + (KMAJOR ? gr * ld + gk : gk * ld + gr) : p, in);
     }
 }
 
-template <typename T, bool AK, bool BK, int ACT>
-__global__ void __launch_bounds__(kSimtThreads) simt_gemm_kernel(GemmArgs a)
+template <int TILE, bool AK, bool BK, int ACT>
+__global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
 {
-    __shared__ float sa[kDepth][kTile + 4], sb[kDepth][kTile + 4];
+    using S         = SimtShape<TILE>;
+    constexpr int M = TILE / 16;   // results per thread and direction: rows ty 4 + {0..3} (+ 64), columns alike
+    extern __shared__ __align__(16) float simt_smem[];
     pdl_launch_dependents();
+    uint32_t splits;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+    const uint32_t rank   = tc::cluster_rank();
+    const int64_t tile    = blockIdx.x / splits;
+    const int64_t tiles_j = (a.cols + TILE - 1) / TILE;
+    const int64_t i0 = tile / tiles_j * TILE, j0 = tile % tiles_j * TILE;
+    const int64_t slices = (a.depth + kDepth - 1) / kDepth;
+    const int64_t s0 = slices * rank / splits, s1 = slices * (rank + 1) / splits;
+    const float* pa = (const float*) a.a;
+    const float* pb = (const float*) a.b;
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const uint32_t base = tc::smem_addr(simt_smem);
+    auto load = [&](int64_t slice) {
+        if (slice < s1)
+        {
+            const uint32_t dst = base + (uint32_t) ((slice - s0) % S::kStages) * 2 * S::kSlice * 4;
+            simt_load<TILE, AK>(pa, a.lda, a.rows, a.depth, i0, slice * kDepth, dst);
+            simt_load<TILE, BK>(pb, a.ldb, a.cols, a.depth, j0, slice * kDepth, dst + S::kSlice * 4);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     pdl_wait();
-    const int64_t tiles_j = (a.cols + kTile - 1) / kTile;
-    const int64_t i0 = (int64_t) (blockIdx.x / tiles_j) * kTile, j0 = (int64_t) (blockIdx.x % tiles_j) * kTile;
-    const int ti = (threadIdx.x / 16) * 4, tj = (threadIdx.x % 16) * 4;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < a.depth; k0 += kDepth)
+    f32x2_t acc[M][M / 2];
+#pragma unroll
+    for (int u = 0; u < M; ++u)
+#pragma unroll
+        for (int v = 0; v < M / 2; ++v)
+            acc[u][v] = pair(0.f, 0.f);
+    for (int s = 0; s < S::kStages - 1; ++s)
+        load(s0 + s);
+    for (int64_t slice = s0; slice < s1; ++slice)
     {
-        simt_load<T, AK>((const T*) a.a, a.lda, a.rows, a.depth, i0, k0, sa);
-        simt_load<T, BK>((const T*) a.b, a.ldb, a.cols, a.depth, j0, k0, sb);
-        __syncthreads();
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+        __syncthreads();   // the slice is there, and everybody is done with the one that is overwritten next
+        load(slice + S::kStages - 1);
+        const float* sa = simt_smem + ((slice - s0) % S::kStages) * 2 * S::kSlice;
+        const float* sb = sa + S::kSlice;
 #pragma unroll
         for (int kk = 0; kk < kDepth; ++kk)
         {
-            float av[4], bv[4];
+            float av[M], bv[M];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int h = 0; h < M / 4; ++h)
             {
-                av[u] = sa[kk][ti + u];
-                bv[u] = sb[kk][tj + u];
+                *reinterpret_cast<float4*>(av + 4 * h) = *reinterpret_cast<const float4*>(sa + kk * S::kPitch + 64 * h + ty * 4);
+                *reinterpret_cast<float4*>(bv + 4 * h) = *reinterpret_cast<const float4*>(sb + kk * S::kPitch + 64 * h + tx * 4);
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < M; ++u)
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    acc[u][v] = fmaf(av[u], bv[v], acc[u][v]);
+                for (int v = 0; v < M / 2; ++v)
+                    acc[u][v] = fma2(pair(av[u], av[u]), pair(bv[2 * v], bv[2 * v + 1]), acc[u][v]);
         }
-        __syncthreads();
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    auto finish = [&](float z, int64_t i, int64_t j) {
+        if (i >= a.rows || j >= a.cols)
+            return;
+        if (a.bias)
+            z += ((const float*) a.bias)[j];
+        if (a.z)
+            ((float*) a.z)[i * a.ldz + j] = z;
+        float y = act_value<ACT, false>(z);
+        if (a.residual)
+            y += ((const float*) a.residual)[i * a.ldr + j];
+        ((float*) a.out)[i * a.ldo + j] = y;
+    };
+    if (splits == 1)
+    {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < M; ++u)
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
+            for (int v = 0; v < M / 2; ++v)
+            {
+                float lo, hi;
+                unpair(acc[u][v], lo, hi);
+                const int64_t i = i0 + u / 4 * 64 + ty * 4 + u % 4, j = j0 + v / 2 * 64 + tx * 4 + v % 2 * 2;
+                finish(lo, i, j);
+                finish(hi, i, j + 1);
+            }
+        return;
+    }
+    __syncthreads();   // the operands are no longer needed
+#pragma unroll
+    for (int u = 0; u < M; ++u)
+#pragma unroll
+        for (int v = 0; v < M / 2; ++v)
         {
-            const int64_t i = i0 + ti + u, j = j0 + tj + v;
-            if (i >= a.rows || j >= a.cols)
-                continue;
-            float z = acc[u][v];
-            if (a.bias)
-                z += to_f32(((const T*) a.bias)[j]);
-            if (a.z)
-                ((T*) a.z)[i * a.ldz + j] = from_f32<T>(z);
-            float y = act_value<ACT, false>(z);
-            if (a.residual)
-                y += to_f32(((const T*) a.residual)[i * a.ldr + j]);
-            ((T*) a.out)[i * a.ldo + j] = from_f32<T>(y);
+            float lo, hi;
+            unpair(acc[u][v], lo, hi);
+            float* at = simt_smem + (u / 4 * 64 + ty * 4 + u % 4) * TILE + v / 2 * 64 + tx * 4 + v % 2 * 2;
+            at[0]     = lo;
+            at[1]     = hi;
         }
+    tc::cluster_sync();
+    const int e0 = TILE * TILE / kSimtThreads * (int) rank / (int) splits, e1 = TILE * TILE / kSimtThreads * (int) (rank + 1) / (int) splits;
+    for (int s = e0; s < e1; ++s)
+    {
+        const int e = s * kSimtThreads + threadIdx.x;
+        float z     = 0.f;
+        for (uint32_t r = 0; r < splits; ++r)   // always in this order: the same bits on every run
+            z += tc::ld_cluster(tc::map_to(base + e * 4, r));
+        finish(z, i0 + e / TILE, j0 + e % TILE);
+    }
+    tc::cluster_sync();   // nobody leaves while its partial tile may be read
 }
 
-template <typename T, bool AK, bool BK>
-int simt_gemm(const GemmArgs& a, cudaStream_t st)
+template <int TILE, bool AK, bool BK>
+int simt_gemm(const GemmArgs& a, int splits, cudaStream_t st)
 {
-    const int64_t grid = ((a.rows + kTile - 1) / kTile) * ((a.cols + kTile - 1) / kTile);
+    const int64_t grid = ((a.rows + TILE - 1) / TILE) * ((a.cols + TILE - 1) / TILE) * splits;
     if (grid > 0x7fffffff)
         return AQ_ERR_TOO_LARGE;
-    return with_activation(a.act, [&](auto act) {
-        const cudaError_t e =
-            launch_pdl(simt_gemm_kernel<T, AK, BK, decltype(act)::value>, dim3((unsigned) grid), kSimtThreads, 0, st, a);
+    return with_activation(a.act, [&](auto act) -> int {
+        auto kernel   = simt_gemm_kernel<TILE, AK, BK, decltype(act)::value>;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SimtShape<TILE>::kSmem);
+        if (e == cudaSuccess)
+            e = launch_cluster(kernel, (unsigned) grid, splits, kSimtThreads, SimtShape<TILE>::kSmem, st, a);
         note_launch();
         return e == cudaSuccess ? AQ_OK : cuda_fail(e);
     });
 }
 
-template <typename T>
+template <bool AK, bool BK>
 int simt_dispatch(const GemmArgs& a, cudaStream_t st)
 {
+    // Two CTAs per SM.  128 x 128 tiles need half the shared memory traffic per product; 64 x 64 ones with the depth
+    // split come closer to filling the GPU when there are fewer than that many large ones.
+    const int64_t large = ((a.rows + 127) / 128) * ((a.cols + 127) / 128);
+    if (large >= 2 * kNumSMs)
+        return simt_gemm<128, AK, BK>(a, 1, st);
+    const int64_t small = ((a.rows + 63) / 64) * ((a.cols + 63) / 64), slices = (a.depth + kDepth - 1) / kDepth;
+    int64_t splits = 4 * kNumSMs / small;
+    splits         = splits < slices / 4 ? splits : slices / 4;
+    return simt_gemm<64, AK, BK>(a, (int) (splits < 1 ? 1 : splits > 8 ? 8 : splits), st);
+}
+
+int simt_any(const GemmArgs& a, cudaStream_t st)
+{
     if (a.a_kmajor && a.b_kmajor)
-        return simt_gemm<T, true, true>(a, st);
+        return simt_dispatch<true, true>(a, st);
     if (a.a_kmajor)
-        return simt_gemm<T, true, false>(a, st);
-    return simt_gemm<T, false, false>(a, st);
+        return simt_dispatch<true, false>(a, st);
+    return simt_dispatch<false, false>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -320,7 +417,7 @@ int grad_z(const GradZArgs& a, cudaStream_t st)
 int gemm(const GemmArgs& a, cudaStream_t st)
 {
     if (a.dtype == AQ_F32)
-        return simt_dispatch<float>(a, st);
+        return simt_any(a, st);
     if (a.depth == 0)
     {
         const cudaError_t e = cudaMemset2DAsync(a.out, (size_t) a.ldo * 2, 0, (size_t) a.cols * 2, (size_t) a.rows, st);

@@ -237,4 +237,26 @@ __device__ __forceinline__ void stuck_exit(volatile int* stuck, int* flag)
     }
 }
 }   // namespace tc
+
+// launch_pdl with clusters of `cluster` CTAs
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, int cluster, unsigned block, size_t smem,
+                                  cudaStream_t st, const Args&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim            = dim3(grid);
+    cfg.blockDim           = dim3(block);
+    cfg.dynamicSmemBytes   = smem;
+    cfg.stream             = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id                                         = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x                           = cluster;
+    attr[1].val.clusterDim.y                           = 1;
+    attr[1].val.clusterDim.z                           = 1;
+    cfg.attrs                                          = attr;
+    cfg.numAttrs                                       = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
 }   // namespace aq

@@ -185,7 +185,7 @@ __device__ __forceinline__ void column_chunk(const TcArgs& p, float (&acc)[N], i
 }
 
 template <typename T, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(128 + 32 * kPairWarps, 1)
+__global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const TcArgs p)
 {
     using S = PairShape<BN>;
@@ -686,23 +686,8 @@ int launch(Kernel kernel, int64_t grid, int cluster, int threads, int smem, cuda
     if (grid > 0x7fffffff)
         return AQ_ERR_TOO_LARGE;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess)
-        return cuda_fail(e);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim            = dim3((unsigned) grid);
-    cfg.blockDim           = dim3(threads);
-    cfg.dynamicSmemBytes   = smem;
-    cfg.stream             = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-    attr[1].id                                         = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x                           = cluster;
-    attr[1].val.clusterDim.y                           = 1;
-    attr[1].val.clusterDim.z                           = 1;
-    cfg.attrs                                          = attr;
-    cfg.numAttrs                                       = cluster > 0 ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, p);
+    if (e == cudaSuccess)
+        e = launch_cluster(kernel, (unsigned) grid, cluster, threads, smem, st, ma, mb, p);
     note_launch();
     return e == cudaSuccess ? AQ_OK : cuda_fail(e);
 }
@@ -725,7 +710,7 @@ int run_pair(const GemmArgs& a, cudaStream_t st)
     if (tiles > 0x3fffffff)
         return AQ_ERR_TOO_LARGE;
     const int64_t pairs = tiles < kNumSMs / 2 ? tiles : kNumSMs / 2;
-    return launch(pair_kernel<T, BN>, 2 * pairs, 0, 128 + 32 * kPairWarps, PairShape<BN>::kSmem, st, ma, mb, p);
+    return launch(pair_kernel<T, BN>, 2 * pairs, 2, 128 + 32 * kPairWarps, PairShape<BN>::kSmem, st, ma, mb, p);
 }
 
 template <typename T, int BN>

@@ -26,8 +26,9 @@ struct SimtShape
 {
     static constexpr int kPitch  = TILE + 4;   // [k][row]; the pad spreads the turned copies over the banks
     static constexpr int kStages = 4;
-    static constexpr int kSlice  = kDepth * kPitch;                     // floats of one operand
-    static constexpr int kSmem   = kStages * 2 * kSlice * 4;
+    static constexpr int kOffB   = kDepth * kPitch;              // floats
+    static constexpr int kStage  = kOffB + kDepth * kPitch;
+    static constexpr int kSmem   = kStages * kStage * 4;
     static_assert(TILE * TILE * 4 <= kSmem, "the partial tile takes the place of the operands");
 };
 
@@ -36,20 +37,23 @@ __device__ __forceinline__ void copy_async4(uint32_t dst, const float* src, bool
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
 
-// Slice of TILE rows x 16 k from row0, k0; what lies outside the matrix becomes 0 (the address then is the matrix itself).
+// Slice of TILE rows x 16 k, element (r, c) to dst + c * kPitch + r; what lies outside the matrix (rows beyond
+// `rows`, k beyond `depth`) becomes 0, and the address then is the start of the slice.
 template <int TILE, bool KMAJOR>
-__device__ __forceinline__ void simt_load(const float* p, int64_t ld, int64_t rows, int64_t k_end, int64_t row0, int64_t k0,
-                                          uint32_t dst)
+__device__ __forceinline__ void simt_load(const float* p, int64_t ld, int rows, int depth, uint32_t dst)
 {
+    constexpr int PITCH = SimtShape<TILE>::kPitch;
+    constexpr int STEP = KMAJOR ? kSimtThreads / kDepth : kSimtThreads / TILE;   // rows, or k, from one copy to the next
+    const int r = KMAJOR ? threadIdx.x / kDepth : threadIdx.x % TILE, c = KMAJOR ? threadIdx.x % kDepth : threadIdx.x / TILE;
+    const float* src = p + (KMAJOR ? r * ld + c : c * ld + r);
+    uint32_t at      = dst + (c * PITCH + r) * 4;
 #pragma unroll
     for (int s = 0; s < TILE * kDepth / kSimtThreads; ++s)
     {
-        const int e = s * kSimtThreads + threadIdx.x;
-        const int r = KMAJOR ? e / kDepth : e % TILE;
-        const int c = KMAJOR ? e % kDepth : e / TILE;
-        const int64_t gr = row0 + r, gk = k0 + c;
-        const bool in = gr < rows && gk < k_end;
-        copy_async4(dst + (c * SimtShape<TILE>::kPitch + r) * 4, in ? p + (KMAJOR ? gr * ld + gk : gk * ld + gr) : p, in);
+        const bool in = KMAJOR ? r + s * STEP < rows && c < depth : r < rows && c + s * STEP < depth;
+        copy_async4(at, in ? src : p, in);
+        src += STEP * ld;
+        at += STEP * (KMAJOR ? 1 : PITCH) * 4;
     }
 }
 
@@ -72,12 +76,16 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
     const float* pb = (const float*) a.b;
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     const uint32_t base = tc::smem_addr(simt_smem);
+    const int rows_left = a.rows - i0 < TILE ? (int) (a.rows - i0) : TILE, cols_left = a.cols - j0 < TILE ? (int) (a.cols - j0) : TILE;
     auto load = [&](int64_t slice) {
         if (slice < s1)
         {
-            const uint32_t dst = base + (uint32_t) ((slice - s0) % S::kStages) * 2 * S::kSlice * 4;
-            simt_load<TILE, AK>(pa, a.lda, a.rows, a.depth, i0, slice * kDepth, dst);
-            simt_load<TILE, BK>(pb, a.ldb, a.cols, a.depth, j0, slice * kDepth, dst + S::kSlice * 4);
+            const uint32_t dst = base + (uint32_t) ((slice - s0) % S::kStages) * S::kStage * 4;
+            const int64_t k0   = slice * kDepth;
+            const int left     = a.depth - k0 < kDepth ? (int) (a.depth - k0) : kDepth;
+            simt_load<TILE, AK>(pa + (AK ? i0 * a.lda + k0 : k0 * a.lda + i0), a.lda, rows_left, left, dst);
+            simt_load<TILE, BK>(pb + (BK ? j0 * a.ldb + k0 : k0 * a.ldb + j0), a.ldb, cols_left, left,
+                                               dst + S::kOffB * 4);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -95,23 +103,27 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
         __syncthreads();   // the slice is there, and everybody is done with the one that is overwritten next
         load(slice + S::kStages - 1);
-        const float* sa = simt_smem + ((slice - s0) % S::kStages) * 2 * S::kSlice;
-        const float* sb = sa + S::kSlice;
+        const float* sa = simt_smem + ((slice - s0) % S::kStages) * S::kStage + ty * 4;
+        const float* sb = simt_smem + ((slice - s0) % S::kStages) * S::kStage + S::kOffB + tx * 4;
 #pragma unroll
         for (int kk = 0; kk < kDepth; ++kk)
         {
-            float av[M], bv[M];
+            float av[M];
+            ulonglong2 bv[M / 4];   // the register pairs (b0, b1), (b2, b3)
 #pragma unroll
             for (int h = 0; h < M / 4; ++h)
             {
-                *reinterpret_cast<float4*>(av + 4 * h) = *reinterpret_cast<const float4*>(sa + kk * S::kPitch + 64 * h + ty * 4);
-                *reinterpret_cast<float4*>(bv + 4 * h) = *reinterpret_cast<const float4*>(sb + kk * S::kPitch + 64 * h + tx * 4);
+                *reinterpret_cast<float4*>(av + 4 * h) = *reinterpret_cast<const float4*>(sa + kk * S::kPitch + 64 * h);
+                bv[h] = *reinterpret_cast<const ulonglong2*>(sb + kk * S::kPitch + 64 * h);
             }
 #pragma unroll
             for (int u = 0; u < M; ++u)
+            {
+                const f32x2_t a2 = pair(av[u], av[u]);
 #pragma unroll
                 for (int v = 0; v < M / 2; ++v)
-                    acc[u][v] = fma2(pair(av[u], av[u]), pair(bv[2 * v], bv[2 * v + 1]), acc[u][v]);
+                    acc[u][v] = fma2(a2, v % 2 ? bv[v / 2].y : bv[v / 2].x, acc[u][v]);
+            }
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");

@@ -5,6 +5,8 @@
 // depth split over a cluster -- for few rows, where the time is reading B once, and for products too small to
 // fill the GPU with large tiles.  Both read either operand as rows over k or as columns (GemmArgs), so the forward
 // product and the two of the backward pass need no transposed copies.
+#include <atomic>
+
 #include "activation.cuh"
 #include "kernels.h"
 #include "tensor_core.cuh"
@@ -730,35 +732,89 @@ int run_slim(const GemmArgs& a, int splits, cudaStream_t st)
     return launch(slim_kernel<T, BN>, (int64_t) p.tiles_i * p.tiles_j * splits, splits, 192, SlimShape<BN>::kSmem, st, ma, mb, p);
 }
 
-// CTAs of a cluster that share the depth: enough CTAs for two per SM, at least 4 blocks of 64 k each, at most 8
-int slim_splits(int64_t tiles, int64_t k_blocks)
+// Clusters of `splits` CTAs of slim_kernel that the current device holds at once (a cluster lives inside one GPC, so this
+// is less than the SMs' room divided by the cluster: 30 of the 37 that 296 CTAs by eight would be).  Asked once.
+template <typename T, int BN>
+int resident_clusters(int splits)
 {
-    int64_t s = 2 * kNumSMs / tiles;
-    s         = s < k_blocks / 4 ? s : k_blocks / 4;
-    return (int) (s < 1 ? 1 : s > 8 ? 8 : s);
+    static std::atomic<int> known[16][9];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16)
+        dev = 0;
+    int n = known[dev][splits].load(std::memory_order_relaxed);
+    if (n == 0)
+    {
+        cudaFuncSetAttribute(slim_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SlimShape<BN>::kSmem);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim            = dim3(splits);
+        cfg.blockDim           = dim3(192);
+        cfg.dynamicSmemBytes   = SlimShape<BN>::kSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id               = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = splits;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs                = attr;
+        cfg.numAttrs             = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, slim_kernel<T, BN>, &cfg) != cudaSuccess || n < 1)
+        {
+            cudaGetLastError();
+            n = 2 * kNumSMs / splits;
+        }
+        known[dev][splits].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// CTAs of a cluster that share the depth, and the blocks of 64 k that the kernel's longest chain of CTAs then walks: a
+// second wave costs more than a larger cluster gains (24 x 11008 -> 4096: 32 tiles by eight CTAs are two waves and 37 us,
+// by seven one).  Filling the pipeline and joining the parts is worth about 8 blocks.
+template <typename T, int BN>
+int64_t slim_plan(int64_t tiles, int64_t k_blocks, int& splits)
+{
+    int64_t best = INT64_MAX;
+    splits       = 1;
+    for (int s = 1; s <= 8 && (s == 1 || k_blocks >= 4 * s); ++s)
+    {
+        const int64_t room = resident_clusters<T, BN>(s);
+        const int64_t cost = (tiles + room - 1) / room * ((k_blocks + s - 1) / s + 8);
+        if (cost < best)
+        {
+            best   = cost;
+            splits = s;
+        }
+    }
+    return best;
 }
 
 template <typename T>
 int tensor_gemm_t(const GemmArgs& a, cudaStream_t st)
 {
-    const int64_t kb = (a.depth + kBlockK - 1) / kBlockK;
-    auto slim_tiles  = [&](int bn) { return (a.rows + bn - 1) / bn * ((a.cols + 127) / 128); };
+    const int64_t kb    = (a.depth + kBlockK - 1) / kBlockK;
+    auto slim_tiles     = [&](int bn) { return (a.rows + bn - 1) / bn * ((a.cols + 127) / 128); };
+    int splits          = 1;
     if (a.rows <= 64 && a.a_kmajor)
     {
         if (a.rows <= 16)
-            return run_slim<T, 16>(a, slim_splits(slim_tiles(16), kb), st);
+        {
+            slim_plan<T, 16>(slim_tiles(16), kb, splits);
+            return run_slim<T, 16>(a, splits, st);
+        }
         if (a.rows <= 32)
-            return run_slim<T, 32>(a, slim_splits(slim_tiles(32), kb), st);
-        return run_slim<T, 64>(a, slim_splits(slim_tiles(64), kb), st);
+        {
+            slim_plan<T, 32>(slim_tiles(32), kb, splits);
+            return run_slim<T, 32>(a, splits, st);
+        }
+        slim_plan<T, 64>(slim_tiles(64), kb, splits);
+        return run_slim<T, 64>(a, splits, st);
     }
-    // Estimated cycles: a stage of pair_kernel costs 512 (BN 256) or 384 (BN 128), one of slim_kernel 512 with one CTA on
-    // the SM; the last term stands for filling the pipeline and the epilogue.
+    // Estimated cycles: a stage of pair_kernel costs 512 (BN 256) or 384 (BN 128), one of slim_kernel 1024 with two CTAs on
+    // the SM; the other term of pair_kernel stands for filling the pipeline and the epilogue.
     auto waves = [](int64_t n, int64_t slots) { return (n + slots - 1) / slots; };
     const int64_t rt = (a.rows + 255) / 256;
     const int64_t p256 = waves(rt * ((a.cols + 255) / 256), kNumSMs / 2) * (kb * 512 + 1500);
     const int64_t p128 = waves(rt * ((a.cols + 127) / 128), kNumSMs / 2) * (kb * 384 + 1000);
-    const int splits   = slim_splits(slim_tiles(128), kb);
-    const int64_t s128 = waves(slim_tiles(128) * splits, 2 * kNumSMs) * ((kb + splits - 1) / splits * 1024 + 3000);
+    const int64_t s128 = slim_plan<T, 128>(slim_tiles(128), kb, splits) * 1024;
     if (s128 < p256 && s128 < p128)
         return run_slim<T, 128>(a, splits, st);
     return p256 <= p128 ? run_pair<T, 256>(a, st) : run_pair<T, 128>(a, st);

@@ -716,7 +716,8 @@ int aq_linear_forward(const void* d_x, int64_t ldx, const void* d_w, int64_t ldw
     if (bad_dtype(dtype) || bad_mnk(m, n, k) || activation < AQ_ACT_NONE || activation > AQ_ACT_SILU ||
         bad_matrix(d_x, ldx, m, k, dtype) || bad_matrix(d_w, ldw, n, k, dtype) || bad_matrix(d_y, ldy, m, n, dtype) ||
         (d_residual && bad_matrix(d_residual, ldr, m, n, dtype)) || (d_z && bad_matrix(d_z, ldz, m, n, dtype)) ||
-        bad_matrix(d_bias, 1, 0, 1, dtype) || unaligned_rows(d_x, ldx, dtype) || unaligned_rows(d_w, ldw, dtype))
+        bad_matrix(d_bias, 1, 0, 1, dtype) ||
+        (m > AQ_LINEAR_FEW_ROWS && (unaligned_rows(d_x, ldx, dtype) || unaligned_rows(d_w, ldw, dtype))))
         return AQ_ERR_INVALID_ARG;
     if (huge(m, n, k))
         return AQ_ERR_TOO_LARGE;

@@ -219,6 +219,247 @@ int simt_any(const GemmArgs& a, cudaStream_t st)
 }
 
 // ------------------------------------------------------------------------------------------------
+// Products for at most 8 rows of A, both operands rows over k: what counts is reading B once, in whole rows.  A CTA takes
+// few_b rows of B and every row of A; its four warps share the depth (2 KB of every row per step with 16-byte accesses)
+// and add up in shared memory.  A comes out of L1.  No alignment is needed: VEC = 1 reads element by element.
+//
+// One row, 4096 -> 11008 in bf16 (90 MB, 13.8 us at the copy bandwidth): 16.8 us, against 23.4 us on the tensor cores'
+// kernel for few rows, which has a pipeline to fill and parts to join between SMs; two rows 19.2 against 23.4, four 27.1
+// against 23.5.  A warp per row group instead of four: 21.7 us; half the loads in flight: the same here, 17.4 against
+// 16.5 us for 11008 -> 4096.
+// ------------------------------------------------------------------------------------------------
+constexpr int kFewRows = AQ_LINEAR_FEW_ROWS;
+
+// 16 bytes as float32 lanes
+template <typename T>
+__device__ __forceinline__ void expand(const uint4& u, f32x2_t (&f)[8 / sizeof(T)])
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (sizeof(T) == 4)
+    {
+        f[0] = pair(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        f[1] = pair(__uint_as_float(w[2]), __uint_as_float(w[3]));
+    }
+    else
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+        {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value)
+                f[q] = pair(__uint_as_float(w[q] << 16), __uint_as_float(w[q] & 0xffff0000u));
+            else
+            {
+                __half2 h;
+                memcpy(&h, &w[q], 4);
+                const float2 v = __half22float2(h);
+                f[q]           = pair(v.x, v.y);
+            }
+        }
+}
+
+// rows of B per warp
+template <int M>
+constexpr int few_b = M <= 4 ? 4 : 2;
+
+template <typename T, int VEC, int M>
+__global__ void __launch_bounds__(128) few_rows_kernel(GemmArgs a)
+{
+    constexpr int kFewB = few_b<M>;
+    __shared__ float sh[4][kFewB * M];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t j0 = (int64_t) blockIdx.x * kFewB;
+    float sums[kFewB][M];
+    if constexpr (VEC > 1)
+    {
+        constexpr int Q = VEC / 2, AHEAD = M == 1 ? 4 : 2, STEP = 128;   // in packets of 16 bytes
+        const uint4* pb[kFewB];
+        const uint4* pa[M];
+#pragma unroll
+        for (int r = 0; r < kFewB; ++r)
+            pb[r] = reinterpret_cast<const uint4*>((const T*) a.b + (j0 + r < a.cols ? j0 + r : a.cols - 1) * a.ldb);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+            pa[m] = reinterpret_cast<const uint4*>((const T*) a.a + (m < a.rows ? m : 0) * a.lda);
+        f32x2_t acc[kFewB][M];
+#pragma unroll
+        for (int r = 0; r < kFewB; ++r)
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                acc[r][m] = pair(0.f, 0.f);
+        auto add = [&](const uint4 (&b)[kFewB], int at) {
+            uint4 x[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                x[m] = pa[m][at];
+            f32x2_t bf[kFewB][Q];
+#pragma unroll
+            for (int r = 0; r < kFewB; ++r)
+                expand<T>(b[r], bf[r]);
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+            {
+                f32x2_t af[Q];
+                expand<T>(x[m], af);
+#pragma unroll
+                for (int r = 0; r < kFewB; ++r)
+#pragma unroll
+                    for (int q = 0; q < Q; ++q)
+                        acc[r][m] = fma2(af[q], bf[r][q], acc[r][m]);
+            }
+        };
+        const int packets = (int) (a.depth / VEC);
+        int at            = threadIdx.x;
+        for (; at + STEP * (AHEAD - 1) < packets; at += STEP * AHEAD)
+        {
+            uint4 b[AHEAD][kFewB];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int r = 0; r < kFewB; ++r)
+                    b[u][r] = pb[r][at + u * STEP];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                add(b[u], at + u * STEP);
+        }
+        for (; at < packets; at += STEP)
+        {
+            uint4 b[kFewB];
+#pragma unroll
+            for (int r = 0; r < kFewB; ++r)
+                b[r] = pb[r][at];
+            add(b, at);
+        }
+#pragma unroll
+        for (int r = 0; r < kFewB; ++r)
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+            {
+                float lo, hi;
+                unpair(acc[r][m], lo, hi);
+                sums[r][m] = lo + hi;
+            }
+    }
+    else
+    {
+        constexpr int AHEAD = 8, STEP = 128;
+        const T* pb[kFewB];
+        const T* pa[M];
+#pragma unroll
+        for (int r = 0; r < kFewB; ++r)
+            pb[r] = (const T*) a.b + (j0 + r < a.cols ? j0 + r : a.cols - 1) * a.ldb;
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+            pa[m] = (const T*) a.a + (m < a.rows ? m : 0) * a.lda;
+#pragma unroll
+        for (int r = 0; r < kFewB; ++r)
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                sums[r][m] = 0.f;
+        auto add = [&](const T (&b)[kFewB], int at) {
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+            {
+                const float x = to_f32(pa[m][at]);
+#pragma unroll
+                for (int r = 0; r < kFewB; ++r)
+                    sums[r][m] = fmaf(x, to_f32(b[r]), sums[r][m]);
+            }
+        };
+        int at = threadIdx.x;
+        for (; at + STEP * (AHEAD - 1) < a.depth; at += STEP * AHEAD)
+        {
+            T b[AHEAD][kFewB];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int r = 0; r < kFewB; ++r)
+                    b[u][r] = pb[r][at + u * STEP];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                add(b[u], at + u * STEP);
+        }
+        for (; at < a.depth; at += STEP)
+        {
+            T b[kFewB];
+#pragma unroll
+            for (int r = 0; r < kFewB; ++r)
+                b[r] = pb[r][at];
+            add(b, at);
+        }
+    }
+    float mine = 0.f;   // lane r M + m ends up with the sum of (r, m)
+#pragma unroll
+    for (int r = 0; r < kFewB; ++r)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+        {
+            float s = sums[r][m];
+#pragma unroll
+            for (int o = 16; o; o >>= 1)
+                s += __shfl_xor_sync(0xffffffffu, s, o);
+            mine = lane == r * M + m ? s : mine;
+        }
+    if (lane < kFewB * M)
+        sh[warp][lane] = mine;
+    __syncthreads();
+    if (warp || lane >= kFewB * M)
+        return;
+    mine = sh[0][lane] + sh[1][lane] + sh[2][lane] + sh[3][lane];
+    const int64_t i = lane % M, j = j0 + lane / M;
+    if (i >= a.rows || j >= a.cols)
+        return;
+    if (a.bias)
+        mine += to_f32(((const T*) a.bias)[j]);
+    if (a.z)
+        ((T*) a.z)[i * a.ldz + j] = from_f32<T>(mine);
+    float v = mine;
+    constexpr bool FAST = sizeof(T) == 2;
+    switch (a.act)
+    {
+    case AQ_ACT_RELU: v = act_value<AQ_ACT_RELU, FAST>(v); break;
+    case AQ_ACT_GELU: v = act_value<AQ_ACT_GELU, FAST>(v); break;
+    case AQ_ACT_GELU_TANH: v = act_value<AQ_ACT_GELU_TANH, FAST>(v); break;
+    case AQ_ACT_SILU: v = act_value<AQ_ACT_SILU, FAST>(v); break;
+    default: break;
+    }
+    if (a.residual)
+        v += to_f32(((const T*) a.residual)[i * a.ldr + j]);
+    ((T*) a.out)[i * a.ldo + j] = from_f32<T>(v);
+}
+
+template <typename T, int VEC, int M>
+int few_rows_m(const GemmArgs& a, cudaStream_t st)
+{
+    const cudaError_t e =
+        launch_pdl(few_rows_kernel<T, VEC, M>, dim3((unsigned) ((a.cols + few_b<M> - 1) / few_b<M>)), 128, 0, st, a);
+    note_launch();
+    return e == cudaSuccess ? AQ_OK : cuda_fail(e);
+}
+
+template <typename T>
+bool few_wide(const GemmArgs& a)
+{
+    constexpr int W = 16 / (int) sizeof(T);
+    return (uintptr_t) a.a % 16 == 0 && (uintptr_t) a.b % 16 == 0 && a.depth % W == 0 && a.ldb % W == 0 &&
+           (a.lda % W == 0 || a.rows == 1);
+}
+
+template <typename T>
+int few_rows(const GemmArgs& a, cudaStream_t st)
+{
+    constexpr int W = 16 / (int) sizeof(T);
+    auto by_rows = [&](auto vec) {
+        constexpr int VEC = decltype(vec)::value;
+        return a.rows == 1 ? few_rows_m<T, VEC, 1>(a, st) :
+               a.rows == 2 ? few_rows_m<T, VEC, 2>(a, st) :
+               a.rows <= 4 ? few_rows_m<T, VEC, 4>(a, st) :
+                             few_rows_m<T, VEC, 8>(a, st);
+    };
+    return few_wide<T>(a) ? by_rows(std::integral_constant<int, W> {}) : by_rows(std::integral_constant<int, 1> {});
+}
+
+// ------------------------------------------------------------------------------------------------
 // dz = dy act'(z) and the partial sums of db.  A thread owns VEC neighbouring columns, a warp 32 VEC of them, and the
 // 8 warps of a CTA take the rows of its band in turn, four of them in flight per thread; the sums stay in registers
 // until the band ends.  Bound by memory (dy and z in, dz out) once the slope costs few instructions: with erff and
@@ -368,16 +609,26 @@ int fold_columns_t(const float* part, int64_t bands, int64_t stride, int64_t col
     return e == cudaSuccess ? AQ_OK : cuda_fail(e);
 }
 
-// Row copies to a pitch the tensor cores can read from; the pad becomes 0.
+// Row copies to a pitch the tensor cores can read from; the pad becomes 0.  Eight elements in flight per thread.
 template <typename T>
 __global__ void __launch_bounds__(256) align_rows_kernel(const T* src, int64_t ld_src, T* dst, int64_t ld_dst, int64_t rows,
                                                          int64_t cols)
 {
     pdl_launch_dependents();
     pdl_wait();
+    constexpr int AT = 8;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
-        for (int64_t c = threadIdx.x; c < ld_dst; c += 256)
-            dst[row * ld_dst + c] = c < cols ? src[row * ld_src + c] : T(0);
+        for (int64_t c = threadIdx.x; c < ld_dst; c += 256 * AT)
+        {
+            T v[AT];
+#pragma unroll
+            for (int u = 0; u < AT; ++u)
+                v[u] = c + 256 * u < cols ? src[row * ld_src + c + 256 * u] : T(0);
+#pragma unroll
+            for (int u = 0; u < AT; ++u)
+                if (c + 256 * u < ld_dst)
+                    dst[row * ld_dst + c + 256 * u] = v[u];
+        }
 }
 
 template <typename T>
@@ -428,6 +679,14 @@ int grad_z(const GradZArgs& a, cudaStream_t st)
 
 int gemm(const GemmArgs& a, cudaStream_t st)
 {
+    if (a.rows <= kFewRows && a.a_kmajor && a.b_kmajor)
+    {
+        if (a.dtype == AQ_F32)
+            return few_rows<float>(a, st);
+        // rows that the tensor cores could read go to them from the third on
+        if (a.rows <= 2 || !few_wide<__half>(a))
+            return a.dtype == AQ_F16 ? few_rows<__half>(a, st) : few_rows<__nv_bfloat16>(a, st);
+    }
     if (a.dtype == AQ_F32)
         return simt_any(a, st);
     if (a.depth == 0)

@@ -23,6 +23,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from .. import ops
+from .._lib import AQ_LINEAR_FEW_ROWS
 
 __all__ = ["linear", "layer_norm", "LayerNorm", "ACTIVATIONS"]
 
@@ -75,7 +76,9 @@ def _new_rows(like: torch.Tensor, m: int, n: int) -> torch.Tensor:
 
 def _linear_forward(x, weight, bias, residual, activation, keep_z):
     n, k = weight.shape
-    xm, wm = ops.aligned_rows(_rows(x, k)), ops.aligned_rows(_rows(weight, k))
+    xm, wm = _rows(x, k), _rows(weight, k)
+    if xm.shape[0] > AQ_LINEAR_FEW_ROWS:
+        xm, wm = ops.aligned_rows(xm), ops.aligned_rows(wm)
     rm = None if residual is None else _rows(residual, n)
     bias = None if bias is None else bias.contiguous()
     m = xm.shape[0]
@@ -119,12 +122,12 @@ class _LinearFn(torch.autograd.Function):
         if need_x:
             dx = dy.new_empty((m, k))
             if m:
-                ops.linear_grad_input(dz, wm, dx)
+                ops.linear_grad_input(dz, ops.aligned_rows(wm), dx)
             if len(ctx.x_shape) != 2:
                 dx = dx.view(ctx.x_shape)
         if need_w:
             dw = dy.new_empty((n, k))
-            ops.linear_grad_weight(dz, xm, dw)
+            ops.linear_grad_weight(dz, ops.aligned_rows(xm), dw)
         return dx, dw, db, grad if need_r else None, None
 
 

@@ -521,8 +521,11 @@ typedef enum
 int aq_align_rows(const void* d_src, int64_t ld_src, void* d_dst, int64_t ld_dst, int dtype, int64_t rows,
                   int64_t cols, void* stream);
 
-/* y = act(x W^T + bias) + residual; x [m, k] and W [n, k] aligned, bias [n] or NULL, residual [m, n] or NULL,
- * y [m, n].  d_z, if not NULL, receives z = x W^T + bias [m, n] for the backward pass, rounded to dtype. */
+/* Up to this many rows aq_linear_forward takes x and W of any alignment. */
+#define AQ_LINEAR_FEW_ROWS 8
+
+/* y = act(x W^T + bias) + residual; x [m, k] and W [n, k] aligned (m > AQ_LINEAR_FEW_ROWS), bias [n] or NULL,
+ * residual [m, n] or NULL, y [m, n].  d_z, if not NULL, receives z = x W^T + bias [m, n] for the backward pass, rounded to dtype. */
 int aq_linear_forward(const void* d_x, int64_t ldx, const void* d_w, int64_t ldw, const void* d_bias,
                       const void* d_residual, int64_t ldr, void* d_y, int64_t ldy, void* d_z, int64_t ldz, int dtype,
                       int64_t m, int64_t n, int64_t k, int activation, void* stream);

@@ -8,7 +8,7 @@ import torch.nn.functional as F
 def test_c_entries_reject_bad_arguments():
     from aimet_b200._lib import lib
     p = 1 << 20   # never read: every call below is refused before a launch
-    fwd = lambda x=p, ldx=64, w=p, ldw=64, b=None, r=None, ldr=0, y=p, ldy=32, z=None, ldz=0, dt=2, m=4, n=32, k=64, act=0: \
+    fwd = lambda x=p, ldx=64, w=p, ldw=64, b=None, r=None, ldr=0, y=p, ldy=32, z=None, ldz=0, dt=2, m=9, n=32, k=64, act=0: \
         lib.aq_linear_forward(x, ldx, w, ldw, b, r, ldr, y, ldy, z, ldz, dt, m, n, k, act, None)   # noqa: E731
     for bad in (dict(x=None), dict(w=None), dict(y=None), dict(ldx=63), dict(ldw=60), dict(ldy=31), dict(dt=3), dict(dt=-1),
                 dict(m=-1), dict(n=0), dict(k=0), dict(act=5), dict(act=-1), dict(x=p + 2), dict(w=p + 8), dict(ldx=68),

@@ -546,11 +546,11 @@ def test_refusals_on_the_gpu(cuda):
     with pytest.raises(RuntimeError):
         dx.sum().backward()
     # the C entry refuses rows the tensor cores cannot read
-    h = torch.zeros(4, 24, device=cuda, dtype=torch.float16)
-    y = torch.zeros(4, 4, device=cuda, dtype=torch.float16)
-    assert lib.aq_linear_forward(h.data_ptr() + 2, 24, h.data_ptr(), 24, None, None, 0, y.data_ptr(), 4, None, 0, 1, 4, 4, 8,
+    h = torch.zeros(12, 24, device=cuda, dtype=torch.float16)
+    y = torch.zeros(12, 4, device=cuda, dtype=torch.float16)
+    assert lib.aq_linear_forward(h.data_ptr() + 2, 24, h.data_ptr(), 24, None, None, 0, y.data_ptr(), 4, None, 0, 1, 9, 4, 8,
                                  0, None) == -1
-    assert lib.aq_linear_forward(h.data_ptr(), 23, h.data_ptr(), 24, None, None, 0, y.data_ptr(), 4, None, 0, 1, 4, 4, 8,
+    assert lib.aq_linear_forward(h.data_ptr(), 23, h.data_ptr(), 24, None, None, 0, y.data_ptr(), 4, None, 0, 1, 9, 4, 8,
                                  0, None) == -1
 
 

@@ -147,16 +147,17 @@ __device__ __forceinline__ void norm_row(const LayerNormArgs& a, const Pack<T, V
     const f32x2_t m2 = pair(mu, mu);
     s2               = pair(0.f, 0.f);
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
-    {
-        f32x2_t d = sub2(lanes(v, q), m2);
-        // packets beyond the row hold zeros, not the mean: take them out again
-        float lo, hi;
-        unpair(d, lo, hi);
-        const int64_t i = ((int64_t) (2 * q / VEC) * TPR + t) * VEC, j = ((int64_t) ((2 * q + 1) / VEC) * TPR + t) * VEC;
-        d               = pair(i < a.dim ? lo : 0.f, j < a.dim && 2 * q + 1 < PACKS * VEC ? hi : 0.f);
-        s2              = fma2(d, d, s2);
-    }
+    for (int k = 0; k < PACKS; ++k)
+        if (((int64_t) k * TPR + t) * VEC < a.dim)   // what lies beyond the row holds zeros, not the mean
+        {
+            const Pack<T, VEC> one[1] = {v[k]};
+#pragma unroll
+            for (int q = 0; q < (VEC + 1) / 2; ++q)
+            {
+                const f32x2_t d = sub2(lanes(one, q), VEC > 1 ? m2 : pair(mu, 0.f));
+                s2              = fma2(d, d, s2);
+            }
+        }
     const float rstd = 1.f / sqrtf(row_sum2<TPR>(lane_sum(s2), 0.f, red[1]).x / (float) a.dim + a.eps);
     const f32x2_t r2 = pair(rstd, rstd);
     // eight lanes' worth of w and b at a time, so that they need few registers beside the row
@@ -339,15 +340,26 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(4 * PACKS +
     tc::stuck_exit(&stuck_smem, &g_stuck);
 }
 
-// A thread keeps the same columns for every row its group takes; their sums for dw and db stay in its registers.  h and
-// dy w are formed twice, once for the sums of the row and once for dx, from the packets in shared memory.  Each CTA
-// leaves one row of partial sums, part [gridDim.x][2][dim] (TPR = 32: its warps are added up in shared memory first).
+// A thread keeps the same columns for every row its group takes; their sums for dw and db stay in its registers.  Up to
+// 16 columns h and dy w stay there too between the sums of the row and dx; with more they are formed twice, from the
+// packets in shared memory.  16 columns per thread is where the work beside them (reductions, barriers, addresses) stops
+// mattering: 8 columns on 512 threads took 107 us for 16384 x 4096 bf16.  Each CTA leaves one row of partial sums,
+// part [gridDim.x][2][dim] (TPR = 32: its warps are added up in shared memory first).
+template <typename T, int PACKS>
+struct BwdColumns
+{
+    static constexpr int N     = PACKS * (16 / (int) sizeof(T));
+    static constexpr bool KEEP = N <= 16;
+    static constexpr int kRegs = (KEEP ? 4 : 2) * N + 48;
+};
+
 template <typename T, int TPR, int PACKS>
-__global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(2 * PACKS * (16 / (int) sizeof(T)) + 44, RingShape<TPR>::kThreads))
+__global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<T, PACKS>::kRegs, RingShape<TPR>::kThreads))
     norm_bwd_ring_kernel(LayerNormGradArgs a, int stages)
 {
     constexpr int VEC = 16 / (int) sizeof(T), GROUPS = RingShape<TPR>::kGroups;
     constexpr int N = PACKS * VEC, Q = N / 2;
+    constexpr bool KEEP = BwdColumns<T, PACKS>::KEEP;
     extern __shared__ __align__(128) uint8_t ring_smem[];
     __shared__ float4 red[2][8];
     __shared__ int stuck_smem;
@@ -366,8 +378,10 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(2 * PACKS *
     auto request         = [&](int s, int64_t r) {
         ring.request(s, (const T*) a.x + r * a.ldx, (const T*) a.dy + r * a.lddy);
     };
-    // a CTA's stage is requested again one row later than it is read, behind that row's barrier
-    const int ahead = GROUPS > 1 ? stages : stages - 1;
+    // a stage is requested again behind the barrier of the row that it held, or, if dx is formed from it after that barrier,
+    // behind the next row's
+    constexpr bool LATE = !KEEP && GROUPS == 1;
+    const int ahead     = LATE ? stages - 1 : stages;
     if (t == 0)
         for (int s = 0; s < ahead && row + s * stride < a.rows; ++s)
             request(s, row + s * stride);
@@ -395,7 +409,7 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(2 * PACKS *
         }
         const bool ok = ring.wait();
         const uint32_t at_x = ring.at(ring.stage, 0), at_g = ring.at(ring.stage, 1);
-        f32x2_t sg = zero, sgh = zero;
+        f32x2_t sg = zero, sgh = zero, kept_h[KEEP ? Q : 1], kept_g[KEEP ? Q : 1];
 #pragma unroll
         for (int k = 0; k < PACKS; ++k)
         {
@@ -413,13 +427,18 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(2 * PACKS *
                 db[i]            = add2(db[i], dy);
                 sg               = add2(sg, gw);
                 sgh              = fma2(gw, h, sgh);
+                if constexpr (KEEP)
+                {
+                    kept_h[i] = h;
+                    kept_g[i] = gw;
+                }
             }
         }
         float2 sum = row_sum2<TPR>(lane_sum(sg), lane_sum(sgh), red[slot]);
         if (!ok)
             sum.x = __int_as_float(0x7fffffff);
-        if (GROUPS == 1 && t == 0 && row + ahead * stride < a.rows)
-            request(ring.stage == 0 ? stages - 1 : ring.stage - 1, row + ahead * stride);
+        if ((KEEP || LATE) && t == 0 && row + ahead * stride < a.rows)
+            request(LATE ? (ring.stage == 0 ? stages - 1 : ring.stage - 1) : ring.stage, row + ahead * stride);
         if (a.dx)
         {
             // dx = r gw - r mean(g) - h r mean(g h)
@@ -431,16 +450,27 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(2 * PACKS *
                 const int64_t i = ((int64_t) k * TPR + t) * VEC;
                 if (i >= a.dim)
                     continue;
-                Pack<T, VEC> x[1], g[1], o[1], wk[1] = {w[k]};
-                read_row<T, VEC, TPR>(x, at_x + k * TPR * 16, t, a.dim - k * TPR * VEC);
-                read_row<T, VEC, TPR>(g, at_g + k * TPR * 16, t, a.dim - k * TPR * VEC);
+                Pack<T, VEC> o[1];
+                if constexpr (KEEP)
+                {
 #pragma unroll
-                for (int q = 0; q < VEC / 2; ++q)
-                    set_lanes(o, q, fma2(mul2(sub2(lanes(x, q), m2), r2), c12, fma2(mul2(lanes(g, q), lanes(wk, q)), r2, c02)));
+                    for (int q = 0; q < VEC / 2; ++q)
+                        set_lanes(o, q, fma2(kept_h[k * (VEC / 2) + q], c12, fma2(kept_g[k * (VEC / 2) + q], r2, c02)));
+                }
+                else
+                {
+                    Pack<T, VEC> x[1], g[1], wk[1] = {w[k]};
+                    read_row<T, VEC, TPR>(x, at_x + k * TPR * 16, t, a.dim - k * TPR * VEC);
+                    read_row<T, VEC, TPR>(g, at_g + k * TPR * 16, t, a.dim - k * TPR * VEC);
+#pragma unroll
+                    for (int q = 0; q < VEC / 2; ++q)
+                        set_lanes(o, q,
+                                  fma2(mul2(sub2(lanes(x, q), m2), r2), c12, fma2(mul2(lanes(g, q), lanes(wk, q)), r2, c02)));
+                }
                 store_pack<T, VEC>((T*) a.dx + row * a.dim + i, o[0]);
             }
         }
-        if (GROUPS > 1)
+        if (!KEEP && !LATE)
         {
             __syncwarp();
             if (t == 0 && row + ahead * stride < a.rows)
@@ -740,6 +770,35 @@ int with_row_shape(int64_t packets, F&& f)
     AQ_SHAPE(512, 24)
     return AQ_ERR_TOO_LARGE;
 }
+// the same for the backward ring: 16 columns per thread where the row's length allows; up to 1024 elements of 16 bits a
+// warp takes the row alone
+template <typename T, typename F>
+int with_sums_shape(int64_t packets, F&& f)
+{
+    constexpr int MAX_PACKS = 8;
+    AQ_SHAPE(32, 1)
+    AQ_SHAPE(32, 2)
+    if constexpr (sizeof(T) == 2)
+    {
+        AQ_SHAPE(32, 3)
+        AQ_SHAPE(32, 4)
+        AQ_SHAPE(128, 2)
+        AQ_SHAPE(256, 2)
+        AQ_SHAPE(512, 2)
+        AQ_SHAPE(512, 3)
+        AQ_SHAPE(512, 4)
+    }
+    else
+    {
+        AQ_SHAPE(32, 4)
+        AQ_SHAPE(128, 4)
+        AQ_SHAPE(256, 4)
+        AQ_SHAPE(512, 4)
+        AQ_SHAPE(512, 6)
+        AQ_SHAPE(512, 8)
+    }
+    return AQ_ERR_TOO_LARGE;
+}
 // the same for the forward ring, which keeps no sums: fewer threads and more packets per row
 template <int MAX_PACKS, typename F>
 int with_ring_shape(int64_t packets, F&& f)
@@ -844,11 +903,10 @@ template <typename T>
 int norm_bwd_wide(const LayerNormGradArgs& a, cudaStream_t st)
 {
     constexpr int VEC = 16 / (int) sizeof(T);
-    // at most 32 columns per thread (64 running sums)
-    return with_row_shape<32 / VEC>(a.dim / VEC, [&](auto tpr, auto packs) -> int {
+    return with_sums_shape<T>(a.dim / VEC, [&](auto tpr, auto packs) -> int {
         constexpr int TPR = decltype(tpr)::value, PACKS = decltype(packs)::value;
         using S     = RingShape<TPR>;
-        int ctas    = ctas_for(2 * PACKS * VEC + 44, S::kThreads);
+        int ctas    = ctas_for(BwdColumns<T, PACKS>::kRegs, S::kThreads);
         const int n = ring_stages(2 * a.dim * (int64_t) sizeof(T), S::kGroups, ctas);
         if (n == 0)
             return AQ_ERR_TOO_LARGE;

@@ -23,13 +23,20 @@ namespace
 {
 constexpr int kLoopThreads = 256;
 
-// Sum of two floats over the TPR threads of a row (a warp, or the whole CTA); every thread gets both.  Consecutive calls
+// CTAs per SM that registers allow when a thread needs about `regs`
+constexpr int ctas_for(int regs, int threads)
+{
+    const int n = 65536 / ((regs + 7) / 8 * 8 * threads);
+    return n < 1 ? 1 : n > 8 ? 8 : n;
+}
+
+// Sum of two floats over the TPR threads of a row (part of a warp, a warp, or the whole CTA); every thread gets both.  Consecutive calls
 // of a CTA have to use different `red` (one barrier each).
 template <int TPR>
 __device__ __forceinline__ float2 row_sum2(float a, float b, float4 (&red)[8])
 {
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
+    for (int o = TPR < 32 ? TPR / 2 : 16; o; o >>= 1)
     {
         a += __shfl_xor_sync(0xffffffffu, a, o);
         b += __shfl_xor_sync(0xffffffffu, b, o);
@@ -135,7 +142,7 @@ __device__ __forceinline__ void store_row(const Pack<T, VEC> (&p)[PACKS], T* row
 // w and b come out of L1.  The arithmetic runs two float32 lanes per instruction.
 template <typename T, int VEC, int TPR, int PACKS, typename F>
 __device__ __forceinline__ void norm_row(const LayerNormArgs& a, const Pack<T, VEC> (&v)[PACKS], int64_t row, int t,
-                                         float4 (&red)[2][8], F&& after_read)
+                                         float4 (&red)[2][8], bool live, F&& after_read)
 {
     constexpr int Q = (PACKS * VEC + 1) / 2;
     f32x2_t s2 = pair(0.f, 0.f);
@@ -183,11 +190,11 @@ __device__ __forceinline__ void norm_row(const LayerNormArgs& a, const Pack<T, V
         for (int k = 0; k < AT; ++k)
         {
             const int64_t i = ((int64_t) (k0 + k) * TPR + t) * VEC;
-            if (k0 + k < PACKS && i < a.dim)
+            if (k0 + k < PACKS && i < a.dim && live)
                 store_pack<T, VEC>((T*) a.y + row * a.dim + i, o[k]);
         }
     }
-    if (t == 0 && a.mean)
+    if (t == 0 && a.mean && live)
     {
         a.mean[row] = mu;
         a.rstd[row] = rstd;
@@ -195,7 +202,7 @@ __device__ __forceinline__ void norm_row(const LayerNormArgs& a, const Pack<T, V
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Forward, row in registers.  TPR = 32: four rows per CTA, one per warp.
+// Forward, row in registers.  Up to TPR = 32 a warp takes 32 / TPR neighbouring rows.
 // ------------------------------------------------------------------------------------------------------------------
 template <typename T, int VEC, int TPR, int PACKS>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(LayerNormArgs a)
@@ -206,11 +213,10 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(LayerNo
     pdl_wait();
     const int t       = threadIdx.x % TPR;
     const int64_t row = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR;
-    if (ROWS > 1 && row >= a.rows)
-        return;   // whole warps, and no barrier follows
+    const bool live   = row < a.rows;   // the others of a warp go along with nothing
     Pack<T, VEC> v[PACKS];
-    load_row<T, VEC, TPR>(v, (const T*) a.x + row * a.ldx, t, a.dim, 0.f);
-    norm_row<T, VEC, TPR>(a, v, row, t, red, [] {});
+    load_row<T, VEC, TPR>(v, live ? (const T*) a.x + row * a.ldx : nullptr, t, a.dim, 0.f);
+    norm_row<T, VEC, TPR>(a, v, row, t, red, live, [] {});
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -228,13 +234,6 @@ struct RingShape
     static constexpr int kGroups  = TPR < 128 ? 256 / TPR : 1;
     static_assert(kGroups == 1 || TPR == 32, "a row belongs to a warp or to the CTA");
 };
-
-// CTAs per SM that registers allow when a thread needs about `regs`
-constexpr int ctas_for(int regs, int threads)
-{
-    const int n = 65536 / ((regs + 7) / 8 * 8 * threads);
-    return n < 1 ? 1 : n > 8 ? 8 : n;
-}
 
 // dynamic shared memory: [group][stage][MATRICES][dim] of T, then the barriers [group][stage]
 template <typename T, int MATRICES>
@@ -329,7 +328,7 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(4 * PACKS +
             __syncwarp();
         const int s        = ring.stage;
         const int64_t next = row + stages * stride;
-        norm_row<T, VEC, TPR>(a, v, row, t, red, [&] {
+        norm_row<T, VEC, TPR>(a, v, row, t, red, true, [&] {
             // the barrier inside the row's first sum (or the warp's) is behind every thread: the stage is free
             if (t == 0 && next < a.rows)
                 ring.request(s, x + next * a.ldx);
@@ -511,16 +510,15 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Backward without 16-byte boundaries: as norm_bwd_ring_kernel, but the next row is fetched into registers while the
-// current one is reduced.
+// Backward without 16-byte boundaries, and of short rows: as norm_bwd_ring_kernel, but the next row is fetched into
+// registers while the current one is reduced.  Up to TPR = 32 a warp takes 32 / TPR neighbouring rows at a time.
 // ------------------------------------------------------------------------------------------------------------------
 template <int TPR, int COLUMNS>
 struct BwdShape
 {
     static constexpr int kThreads = TPR < 128 ? 256 : TPR;
     static constexpr int kRows    = TPR < 128 ? 256 / TPR : 1;
-    // resident CTAs per SM that the registers allow: about 5 per column and 32 more
-    static constexpr int kCtas = 65536 / ((5 * COLUMNS + 40) * kThreads) < 1 ? 1 : 65536 / ((5 * COLUMNS + 40) * kThreads);
+    static constexpr int kCtas    = ctas_for(5 * COLUMNS + 40, kThreads);
 };
 
 template <typename T, int VEC, int TPR, int PACKS>
@@ -530,7 +528,7 @@ __global__ void __launch_bounds__(BwdShape<TPR, PACKS * VEC>::kThreads, BwdShape
     constexpr int ROWS = BwdShape<TPR, PACKS * VEC>::kRows;
     constexpr int N = PACKS * VEC, Q = (N + 1) / 2;
     constexpr bool AHEAD = N <= 16;   // with more columns the registers of 512 threads do not hold the next row
-    static_assert(ROWS == 1 || TPR == 32, "a row belongs to a warp or to the CTA");
+    static_assert(ROWS == 1 || TPR <= 32, "a row belongs to (part of) a warp or to the CTA");
     __shared__ float4 red[2][8];
     __shared__ float sums[ROWS > 1 ? ROWS : 1][ROWS > 1 ? TPR * N + 1 : 1];
     pdl_launch_dependents();
@@ -544,16 +542,18 @@ __global__ void __launch_bounds__(BwdShape<TPR, PACKS * VEC>::kThreads, BwdShape
         dw[q] = db[q] = zero;
     Pack<T, VEC> x[PACKS], g[PACKS];
     float mu = 0.f, rstd = 0.f;
-    auto fetch = [&](int64_t row) {
-        mu   = a.mean[row];
-        rstd = a.rstd[row];
-        load_row<T, VEC, TPR>(x, (const T*) a.x + row * a.ldx, t, a.dim, 0.f);
-        load_row<T, VEC, TPR>(g, (const T*) a.dy + row * a.lddy, t, a.dim, 0.f);   // no part in any sum beyond the row
+    auto fetch = [&](int64_t row) {   // beyond the last row, and beyond a row's end: no part in any sum
+        const bool live = row < a.rows;
+        mu              = live ? a.mean[row] : 0.f;
+        rstd            = live ? a.rstd[row] : 0.f;
+        load_row<T, VEC, TPR>(x, live ? (const T*) a.x + row * a.ldx : nullptr, t, a.dim, 0.f);
+        load_row<T, VEC, TPR>(g, live ? (const T*) a.dy + row * a.lddy : nullptr, t, a.dim, 0.f);
     };
-    int64_t row = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR;
-    if (AHEAD && row < a.rows)
+    int64_t row     = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR;
+    const int above = TPR < 32 ? (threadIdx.x & 31) / TPR : 0;   // rows of this warp above this one
+    if (AHEAD)
         fetch(row);
-    for (int slot = 0; row < a.rows; row += stride, slot ^= 1)
+    for (int slot = 0; row - above < a.rows; row += stride, slot ^= 1)
     {
         if (!AHEAD)
             fetch(row);
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(BwdShape<TPR, PACKS * VEC>::kThreads, BwdShape
             h[q]             = hq;
             gw[q]            = gq;
         }
-        if (AHEAD && row + stride < a.rows)
+        if (AHEAD && row + stride - above < a.rows)
             fetch(row + stride);
         if (!a.dx)
             continue;
@@ -587,7 +587,8 @@ __global__ void __launch_bounds__(BwdShape<TPR, PACKS * VEC>::kThreads, BwdShape
 #pragma unroll
         for (int q = 0; q < Q; ++q)
             set_lanes(o, q, fma2(h[q], c12, fma2(gw[q], r2, c02)));
-        store_row<T, VEC, TPR>(o, (T*) a.dx + row * a.dim, t, a.dim);
+        if (row < a.rows)
+            store_row<T, VEC, TPR>(o, (T*) a.dx + row * a.dim, t, a.dim);
     }
     if (!a.part)
         return;
@@ -751,27 +752,57 @@ __global__ void __launch_bounds__(256) norm_param_kernel(LayerNormGradArgs a, in
             return f(std::integral_constant<int, TPR> {}, std::integral_constant<int, PACKS> {});
 
 // f(TPR, PACKS) for the first shape that holds `packets` packets, AQ_ERR_TOO_LARGE (and no call) when none does.
-// MAX_PACKS bounds the registers a thread gives to its columns.
+// Rows in registers, few of them: many threads per row.
 template <int MAX_PACKS, typename F>
 int with_row_shape(int64_t packets, F&& f)
 {
+    AQ_SHAPE(4, 1)
+    AQ_SHAPE(8, 1)
+    AQ_SHAPE(16, 1)
     AQ_SHAPE(32, 1)
     AQ_SHAPE(32, 2)
     AQ_SHAPE(128, 1)
     AQ_SHAPE(256, 1)
     AQ_SHAPE(512, 1)
     AQ_SHAPE(512, 2)
-    AQ_SHAPE(512, 3)
     AQ_SHAPE(512, 4)
-    AQ_SHAPE(512, 6)
     AQ_SHAPE(512, 8)
-    AQ_SHAPE(512, 12)
     AQ_SHAPE(512, 16)
     AQ_SHAPE(512, 24)
     return AQ_ERR_TOO_LARGE;
 }
-// the same for the backward ring: 16 columns per thread where the row's length allows; up to 1024 elements of 16 bits a
-// warp takes the row alone
+// many rows of single elements: fewer threads and more loads in flight
+template <typename F>
+int with_odd_shape(int64_t packets, F&& f)
+{
+    constexpr int MAX_PACKS = 24;
+    AQ_SHAPE(4, 1)
+    AQ_SHAPE(8, 1)
+    AQ_SHAPE(16, 1)
+    AQ_SHAPE(32, 1)
+    AQ_SHAPE(32, 2)
+    AQ_SHAPE(32, 4)
+    AQ_SHAPE(32, 8)
+    AQ_SHAPE(32, 16)
+    AQ_SHAPE(128, 8)
+    AQ_SHAPE(128, 16)
+    AQ_SHAPE(256, 16)
+    AQ_SHAPE(512, 16)
+    AQ_SHAPE(512, 24)
+    return AQ_ERR_TOO_LARGE;
+}
+// short rows of packets
+template <typename F>
+int with_short_shape(int64_t packets, F&& f)
+{
+    constexpr int MAX_PACKS = 1;
+    AQ_SHAPE(4, 1)
+    AQ_SHAPE(8, 1)
+    AQ_SHAPE(16, 1)
+    return AQ_ERR_TOO_LARGE;
+}
+// the same for the backward ring: 16 columns per thread where the row's length allows; a warp takes up to
+// 768 elements of 16 bits or 512 of 32 alone
 template <typename T, typename F>
 int with_sums_shape(int64_t packets, F&& f)
 {
@@ -781,7 +812,7 @@ int with_sums_shape(int64_t packets, F&& f)
     if constexpr (sizeof(T) == 2)
     {
         AQ_SHAPE(32, 3)
-        AQ_SHAPE(32, 4)
+        AQ_SHAPE(128, 1)
         AQ_SHAPE(128, 2)
         AQ_SHAPE(256, 2)
         AQ_SHAPE(512, 2)
@@ -800,9 +831,10 @@ int with_sums_shape(int64_t packets, F&& f)
     return AQ_ERR_TOO_LARGE;
 }
 // the same for the forward ring, which keeps no sums: fewer threads and more packets per row
-template <int MAX_PACKS, typename F>
+template <typename F>
 int with_ring_shape(int64_t packets, F&& f)
 {
+    constexpr int MAX_PACKS = 8;
     AQ_SHAPE(32, 1)
     AQ_SHAPE(32, 2)
     AQ_SHAPE(32, 4)
@@ -853,30 +885,32 @@ template <typename T, int VEC>
 int norm_fwd_v(const LayerNormArgs& a, cudaStream_t st)
 {
     const int64_t packets = (a.dim + VEC - 1) / VEC;
-    if constexpr (VEC > 1)
-    {
-        // the ring pays once its groups take several rows each; before that the plain form starts sooner
-        const int rc = with_ring_shape<8>(packets, [&](auto tpr, auto packs) -> int {
-            constexpr int TPR = decltype(tpr)::value, PACKS = decltype(packs)::value;
-            using S        = RingShape<TPR>;
-            int ctas       = ctas_for(4 * PACKS + 44, S::kThreads);
-            const int n    = ring_stages(a.dim * (int64_t) sizeof(T), S::kGroups, ctas);
-            const int64_t grid = (int64_t) ctas * kNumSMs;
-            if (n == 0 || a.rows < 2 * grid * S::kGroups)
-                return AQ_ERR_TOO_LARGE;
-            return launch_ring(norm_fwd_ring_kernel<T, TPR, PACKS>, a, n, S::kGroups, 1, sizeof(T), grid, S::kThreads, st);
-        });
-        if (rc != AQ_ERR_TOO_LARGE)
-            return rc;
-    }
-    return with_row_shape<VEC == 1 ? 24 : 8>(packets, [&](auto tpr, auto packs) {
+    auto in_registers     = [&](auto tpr, auto packs) {
         constexpr int TPR   = decltype(tpr)::value;
         constexpr int ROWS  = TPR < 128 ? 128 / TPR : 1;
         const cudaError_t e = launch_pdl(norm_fwd_kernel<T, VEC, TPR, decltype(packs)::value>,
                                          dim3((unsigned) ((a.rows + ROWS - 1) / ROWS)), TPR < 128 ? 128 : TPR, 0, st, a);
         note_launch();
         return e == cudaSuccess ? AQ_OK : cuda_fail(e);
-    });
+    };
+    if constexpr (VEC > 1)
+    {
+        // the ring pays once its groups take several rows each, and rows are long enough for a warp; before that the plain
+        // form starts sooner
+        const int rc = packets <= 16 ? AQ_ERR_TOO_LARGE : with_ring_shape(packets, [&](auto tpr, auto packs) -> int {
+            constexpr int TPR = decltype(tpr)::value, PACKS = decltype(packs)::value;
+            using S            = RingShape<TPR>;
+            int ctas           = ctas_for(4 * PACKS + 44, S::kThreads);
+            const int n        = ring_stages(a.dim * (int64_t) sizeof(T), S::kGroups, ctas);
+            const int64_t grid = (int64_t) ctas * kNumSMs;
+            if (n == 0 || a.rows < 2 * grid * S::kGroups)
+                return AQ_ERR_TOO_LARGE;
+            return launch_ring(norm_fwd_ring_kernel<T, TPR, PACKS>, a, n, S::kGroups, 1, sizeof(T), grid, S::kThreads, st);
+        });
+        return rc != AQ_ERR_TOO_LARGE ? rc : with_row_shape<8>(packets, in_registers);
+    }
+    else
+        return a.rows >= 8 * kNumSMs ? with_odd_shape(packets, in_registers) : with_row_shape<24>(packets, in_registers);
 }
 
 template <typename T>
@@ -919,22 +953,24 @@ int norm_bwd_wide(const LayerNormGradArgs& a, cudaStream_t st)
     });
 }
 
-template <typename T>
-int norm_bwd_odd(const LayerNormGradArgs& a, cudaStream_t st)
+template <typename T, int VEC>
+int norm_bwd_registers(const LayerNormGradArgs& a, cudaStream_t st)
 {
-    // at most 24 columns per thread (48 running sums)
-    return with_row_shape<24>(a.dim, [&](auto tpr, auto packs) {
-        using S            = BwdShape<decltype(tpr)::value, decltype(packs)::value>;
+    auto run = [&](auto tpr, auto packs) {
+        using S            = BwdShape<decltype(tpr)::value, decltype(packs)::value * VEC>;
         const int64_t most = bwd_ctas((a.rows + S::kRows - 1) / S::kRows, a.dim);
-        int64_t grid       = (S::kCtas < 4 ? S::kCtas : 4) * kNumSMs;
-        grid               = most < grid ? most : grid;
-        cudaError_t e      = launch_pdl(norm_bwd_kernel<T, 1, decltype(tpr)::value, decltype(packs)::value>,
+        const int64_t grid = most < (int64_t) S::kCtas * kNumSMs ? most : (int64_t) S::kCtas * kNumSMs;
+        cudaError_t e      = launch_pdl(norm_bwd_kernel<T, VEC, decltype(tpr)::value, decltype(packs)::value>,
                                         dim3((unsigned) grid), S::kThreads, 0, st, a);
         note_launch();
         if (e != cudaSuccess)
             return cuda_fail(e);
         return a.part ? fold_columns(a.part, grid, 2 * a.dim, a.dim, a.dw, a.db, a.dtype, st) : AQ_OK;
-    });
+    };
+    if constexpr (VEC > 1)
+        return with_short_shape(a.dim / VEC, run);
+    else
+        return with_odd_shape(a.dim, run);
 }
 
 // Bands of rows of norm_param_kernel: enough of them to fill the GPU, at least 64 rows each.
@@ -951,7 +987,9 @@ template <typename T>
 int norm_bwd_t(const LayerNormGradArgs& a, cudaStream_t st)
 {
     const bool wide = wide_rows<T>(a.x, a.ldx, a.dy, a.lddy, a.w, nullptr, a.dx, a.dim);
-    const int rc    = wide ? norm_bwd_wide<T>(a, st) : norm_bwd_odd<T>(a, st);
+    int rc          = wide ? norm_bwd_registers<T, 16 / (int) sizeof(T)>(a, st) : norm_bwd_registers<T, 1>(a, st);
+    if (rc == AQ_ERR_TOO_LARGE && wide)
+        rc = norm_bwd_wide<T>(a, st);
     if (rc != AQ_ERR_TOO_LARGE)
         return rc;
     if (a.dx)

@@ -8,11 +8,13 @@
 // dy read and dx written once backward.
 //
 // Which kernel takes a call:
-//   norm_fwd_kernel        forward, few rows or rows that do not start on 16-byte boundaries: a row in registers
-//   norm_fwd_ring_kernel   forward, many rows: rows arrive in shared memory by bulk copies, several ahead
-//   norm_bwd_ring_kernel   backward: the same for x and dy, with the sums for dw and db in registers
-//   norm_bwd_kernel        backward without 16-byte boundaries: the next row is fetched into registers
+//   norm_fwd_kernel        forward, a row in the registers of 4 to 512 threads
+//   norm_bwd_ring_kernel   backward: rows arrive in shared memory by bulk copies, several ahead; the sums for dw and db
+//                          stay in registers
+//   norm_bwd_kernel        backward of short rows and of rows without 16-byte boundaries: the next row is fetched into
+//                          registers instead
 //   *_loop_kernel, norm_param_kernel   rows too long for the registers of 512 threads
+// (A forward ring was slower than enough rows in registers: 16384 x 4096 bf16 53 us against 46.)
 #include "common.cuh"
 #include "kernels.h"
 #include "tensor_core.cuh"
@@ -138,11 +140,10 @@ __device__ __forceinline__ void store_row(const Pack<T, VEC> (&p)[PACKS], T* row
     }
 }
 
-// Statistics and result of a row whose packets are in v; `after_read` runs once every thread of the row has v in registers.
-// w and b come out of L1.  The arithmetic runs two float32 lanes per instruction.
-template <typename T, int VEC, int TPR, int PACKS, typename F>
+// Statistics and result of a row whose packets are in v.  w and b come out of L1.  The arithmetic runs two float32 lanes per instruction.
+template <typename T, int VEC, int TPR, int PACKS>
 __device__ __forceinline__ void norm_row(const LayerNormArgs& a, const Pack<T, VEC> (&v)[PACKS], int64_t row, int t,
-                                         float4 (&red)[2][8], bool live, F&& after_read)
+                                         float4 (&red)[2][8], bool live)
 {
     constexpr int Q = (PACKS * VEC + 1) / 2;
     f32x2_t s2 = pair(0.f, 0.f);
@@ -150,7 +151,6 @@ __device__ __forceinline__ void norm_row(const LayerNormArgs& a, const Pack<T, V
     for (int q = 0; q < Q; ++q)
         s2 = add2(s2, lanes(v, q));
     const float mu   = row_sum2<TPR>(lane_sum(s2), 0.f, red[0]).x / (float) a.dim;
-    after_read();
     const f32x2_t m2 = pair(mu, mu);
     s2               = pair(0.f, 0.f);
 #pragma unroll
@@ -216,11 +216,11 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(LayerNo
     const bool live   = row < a.rows;   // the others of a warp go along with nothing
     Pack<T, VEC> v[PACKS];
     load_row<T, VEC, TPR>(v, live ? (const T*) a.x + row * a.ldx : nullptr, t, a.dim, 0.f);
-    norm_row<T, VEC, TPR>(a, v, row, t, red, live, [] {});
+    norm_row<T, VEC, TPR>(a, v, row, t, red, live);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Forward and backward with a ring of rows in shared memory.  One thread of a row's group (a warp, or the CTA) keeps
+// Backward with a ring of rows in shared memory.  One thread of a row's group (a warp, or the CTA) keeps
 // `stages` rows on their way with bulk copies, so that the memory system sees 100 to 200 KB in flight per SM however
 // long the reductions of a row take; with the next row in registers alone it was 16 KB, and the backward pass of 16384
 // x 4096 bf16 took 168 us.  The waits are bounded (see mbar_wait).
@@ -291,52 +291,6 @@ __device__ __forceinline__ void read_row(Pack<T, VEC> (&p)[PACKS], uint32_t row,
                          : "memory");
         memcpy(&p[k], &u, 16);
     }
-}
-
-template <typename T, int TPR, int PACKS>
-__global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(4 * PACKS + 44, RingShape<TPR>::kThreads))
-    norm_fwd_ring_kernel(LayerNormArgs a, int stages)
-{
-    constexpr int VEC = 16 / (int) sizeof(T), GROUPS = RingShape<TPR>::kGroups;
-    extern __shared__ __align__(128) uint8_t ring_smem[];
-    __shared__ float4 red[2][8];
-    __shared__ int stuck_smem;
-    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    Ring<T, 1> ring(tc::smem_addr(ring_smem), GROUPS, group, stages, a.dim, &stuck_smem);
-    pdl_launch_dependents();
-    if (threadIdx.x == 0)
-        stuck_smem = 0;
-    if (t < stages)
-        tc::mbar_init(ring.bars + 8 * t, 1);
-    tc::mbar_init_fence();
-    __syncthreads();
-    pdl_wait();
-    const int64_t stride = (int64_t) gridDim.x * GROUPS;
-    int64_t row          = (int64_t) blockIdx.x * GROUPS + group;
-    const T* x           = (const T*) a.x;
-    if (t == 0)
-        for (int s = 0; s < stages && row + s * stride < a.rows; ++s)
-            ring.request(s, x + (row + s * stride) * a.ldx);
-    for (; row < a.rows; row += stride)
-    {
-        const bool ok = ring.wait();
-        Pack<T, VEC> v[PACKS];
-        read_row<T, VEC, TPR>(v, ring.at(ring.stage, 0), t, a.dim);
-        if (!ok)
-            v[0] = splat<T, VEC>(__int_as_float(0x7fffffff));
-        if (TPR == 32)
-            __syncwarp();
-        const int s        = ring.stage;
-        const int64_t next = row + stages * stride;
-        norm_row<T, VEC, TPR>(a, v, row, t, red, true, [&] {
-            // the barrier inside the row's first sum (or the warp's) is behind every thread: the stage is free
-            if (t == 0 && next < a.rows)
-                ring.request(s, x + next * a.ldx);
-        });
-        ring.advance();
-    }
-    __syncthreads();
-    tc::stuck_exit(&stuck_smem, &g_stuck);
 }
 
 // A thread keeps the same columns for every row its group takes; their sums for dw and db stay in its registers.  Up to
@@ -771,17 +725,16 @@ int with_row_shape(int64_t packets, F&& f)
     AQ_SHAPE(512, 24)
     return AQ_ERR_TOO_LARGE;
 }
-// many rows of single elements: fewer threads and more loads in flight
+// many rows of single elements
 template <typename F>
 int with_odd_shape(int64_t packets, F&& f)
 {
     constexpr int MAX_PACKS = 24;
     AQ_SHAPE(4, 1)
-    AQ_SHAPE(8, 1)
-    AQ_SHAPE(16, 1)
-    AQ_SHAPE(32, 1)
-    AQ_SHAPE(32, 2)
-    AQ_SHAPE(32, 4)
+    AQ_SHAPE(4, 4)
+    AQ_SHAPE(4, 8)
+    AQ_SHAPE(8, 8)
+    AQ_SHAPE(16, 8)
     AQ_SHAPE(32, 8)
     AQ_SHAPE(32, 16)
     AQ_SHAPE(128, 8)
@@ -791,17 +744,38 @@ int with_odd_shape(int64_t packets, F&& f)
     AQ_SHAPE(512, 24)
     return AQ_ERR_TOO_LARGE;
 }
-// short rows of packets
+// many rows of packets
 template <typename F>
-int with_short_shape(int64_t packets, F&& f)
+int with_even_shape(int64_t packets, F&& f)
 {
-    constexpr int MAX_PACKS = 1;
+    constexpr int MAX_PACKS = 8;
     AQ_SHAPE(4, 1)
-    AQ_SHAPE(8, 1)
-    AQ_SHAPE(16, 1)
+    AQ_SHAPE(4, 2)
+    AQ_SHAPE(4, 4)
+    AQ_SHAPE(8, 4)
+    AQ_SHAPE(16, 4)
+    AQ_SHAPE(32, 4)
+    AQ_SHAPE(128, 2)
+    AQ_SHAPE(128, 4)
+    AQ_SHAPE(256, 4)
+    AQ_SHAPE(512, 4)
+    AQ_SHAPE(512, 8)
     return AQ_ERR_TOO_LARGE;
 }
-// the same for the backward ring: 16 columns per thread where the row's length allows; a warp takes up to
+// short rows of packets with sums: at most 16 columns per thread
+template <int MAX_PACKS, typename F>
+int with_short_shape(int64_t packets, F&& f)
+{
+    AQ_SHAPE(4, 1)
+    AQ_SHAPE(4, 2)
+    AQ_SHAPE(4, 4)
+    AQ_SHAPE(8, 2)
+    AQ_SHAPE(8, 4)
+    AQ_SHAPE(16, 2)
+    AQ_SHAPE(16, 4)
+    return AQ_ERR_TOO_LARGE;
+}
+// the backward ring: 16 columns per thread where the row's length allows; a warp takes up to
 // 768 elements of 16 bits or 512 of 32 alone
 template <typename T, typename F>
 int with_sums_shape(int64_t packets, F&& f)
@@ -828,21 +802,6 @@ int with_sums_shape(int64_t packets, F&& f)
         AQ_SHAPE(512, 6)
         AQ_SHAPE(512, 8)
     }
-    return AQ_ERR_TOO_LARGE;
-}
-// the same for the forward ring, which keeps no sums: fewer threads and more packets per row
-template <typename F>
-int with_ring_shape(int64_t packets, F&& f)
-{
-    constexpr int MAX_PACKS = 8;
-    AQ_SHAPE(32, 1)
-    AQ_SHAPE(32, 2)
-    AQ_SHAPE(32, 4)
-    AQ_SHAPE(128, 2)
-    AQ_SHAPE(128, 4)
-    AQ_SHAPE(256, 4)
-    AQ_SHAPE(512, 4)
-    AQ_SHAPE(512, 8)
     return AQ_ERR_TOO_LARGE;
 }
 #undef AQ_SHAPE
@@ -893,24 +852,12 @@ int norm_fwd_v(const LayerNormArgs& a, cudaStream_t st)
         note_launch();
         return e == cudaSuccess ? AQ_OK : cuda_fail(e);
     };
+    // Many rows: few threads per row, so that each has several loads in flight (2048 x 4096 bf16: 8.8 us with 128 threads
+    // and four packets each, 14.7 us with 512 and one).  Few rows: the other way round, one row ends sooner.
     if constexpr (VEC > 1)
-    {
-        // the ring pays once its groups take several rows each, and rows are long enough for a warp; before that the plain
-        // form starts sooner
-        const int rc = packets <= 16 ? AQ_ERR_TOO_LARGE : with_ring_shape(packets, [&](auto tpr, auto packs) -> int {
-            constexpr int TPR = decltype(tpr)::value, PACKS = decltype(packs)::value;
-            using S            = RingShape<TPR>;
-            int ctas           = ctas_for(4 * PACKS + 44, S::kThreads);
-            const int n        = ring_stages(a.dim * (int64_t) sizeof(T), S::kGroups, ctas);
-            const int64_t grid = (int64_t) ctas * kNumSMs;
-            if (n == 0 || a.rows < 2 * grid * S::kGroups)
-                return AQ_ERR_TOO_LARGE;
-            return launch_ring(norm_fwd_ring_kernel<T, TPR, PACKS>, a, n, S::kGroups, 1, sizeof(T), grid, S::kThreads, st);
-        });
-        return rc != AQ_ERR_TOO_LARGE ? rc : with_row_shape<8>(packets, in_registers);
-    }
+        return a.rows > 2 * kNumSMs ? with_even_shape(packets, in_registers) : with_row_shape<8>(packets, in_registers);
     else
-        return a.rows >= 8 * kNumSMs ? with_odd_shape(packets, in_registers) : with_row_shape<24>(packets, in_registers);
+        return a.rows > 2 * kNumSMs ? with_odd_shape(packets, in_registers) : with_row_shape<24>(packets, in_registers);
 }
 
 template <typename T>
@@ -968,7 +915,7 @@ int norm_bwd_registers(const LayerNormGradArgs& a, cudaStream_t st)
         return a.part ? fold_columns(a.part, grid, 2 * a.dim, a.dim, a.dw, a.db, a.dtype, st) : AQ_OK;
     };
     if constexpr (VEC > 1)
-        return with_short_shape(a.dim / VEC, run);
+        return with_short_shape<16 / VEC>(a.dim / VEC, run);
     else
         return with_odd_shape(a.dim, run);
 }

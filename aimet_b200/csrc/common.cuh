@@ -5,6 +5,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "../../include/aimet_b200.h"
 
@@ -243,6 +246,59 @@ __device__ __forceinline__ f32x2_t fma2(f32x2_t a, f32x2_t b, f32x2_t c)
     f32x2_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
+}
+
+// 16 bytes of T as float32 lanes, and back
+template <typename T>
+__device__ __forceinline__ void expand(const uint4& u, f32x2_t (&f)[8 / sizeof(T)])
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (sizeof(T) == 4)
+    {
+        f[0] = pair(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        f[1] = pair(__uint_as_float(w[2]), __uint_as_float(w[3]));
+    }
+    else
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+        {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value)
+                f[q] = pair(__uint_as_float(w[q] << 16), __uint_as_float(w[q] & 0xffff0000u));
+            else
+            {
+                __half2 h;
+                memcpy(&h, &w[q], 4);
+                const float2 v = __half22float2(h);
+                f[q]           = pair(v.x, v.y);
+            }
+        }
+}
+template <typename T>
+__device__ __forceinline__ uint4 compress(const f32x2_t (&f)[8 / sizeof(T)])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < (int) (8 / sizeof(T)); ++q)
+    {
+        float lo, hi;
+        unpair(f[q], lo, hi);
+        if constexpr (sizeof(T) == 4)
+        {
+            w[2 * q]     = __float_as_uint(lo);
+            w[2 * q + 1] = __float_as_uint(hi);
+        }
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+            memcpy(&w[q], &h, 4);
+        }
+        else
+        {
+            const __half2 h = __floats2half2_rn(lo, hi);
+            memcpy(&w[q], &h, 4);
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 }   // namespace aq

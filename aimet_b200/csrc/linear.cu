@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
             z += ((const float*) a.bias)[j];
         if (a.z)
             ((float*) a.z)[i * a.ldz + j] = z;
-        float y = act_value<ACT, false>(z);
+        float y = act_value<ACT>(z);
         if (a.residual)
             y += ((const float*) a.residual)[i * a.ldr + j];
         ((float*) a.out)[i * a.ldo + j] = y;
@@ -229,32 +229,6 @@ int simt_any(const GemmArgs& a, cudaStream_t st)
 // 16.5 us for 11008 -> 4096.
 // ------------------------------------------------------------------------------------------------
 constexpr int kFewRows = AQ_LINEAR_FEW_ROWS;
-
-// 16 bytes as float32 lanes
-template <typename T>
-__device__ __forceinline__ void expand(const uint4& u, f32x2_t (&f)[8 / sizeof(T)])
-{
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    if constexpr (sizeof(T) == 4)
-    {
-        f[0] = pair(__uint_as_float(w[0]), __uint_as_float(w[1]));
-        f[1] = pair(__uint_as_float(w[2]), __uint_as_float(w[3]));
-    }
-    else
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-        {
-            if constexpr (std::is_same<T, __nv_bfloat16>::value)
-                f[q] = pair(__uint_as_float(w[q] << 16), __uint_as_float(w[q] & 0xffff0000u));
-            else
-            {
-                __half2 h;
-                memcpy(&h, &w[q], 4);
-                const float2 v = __half22float2(h);
-                f[q]           = pair(v.x, v.y);
-            }
-        }
-}
 
 // rows of B per warp
 template <int M>
@@ -414,13 +388,12 @@ __global__ void __launch_bounds__(128) few_rows_kernel(GemmArgs a)
     if (a.z)
         ((T*) a.z)[i * a.ldz + j] = from_f32<T>(mine);
     float v = mine;
-    constexpr bool FAST = sizeof(T) == 2;
     switch (a.act)
     {
-    case AQ_ACT_RELU: v = act_value<AQ_ACT_RELU, FAST>(v); break;
-    case AQ_ACT_GELU: v = act_value<AQ_ACT_GELU, FAST>(v); break;
-    case AQ_ACT_GELU_TANH: v = act_value<AQ_ACT_GELU_TANH, FAST>(v); break;
-    case AQ_ACT_SILU: v = act_value<AQ_ACT_SILU, FAST>(v); break;
+    case AQ_ACT_RELU: v = act_value<AQ_ACT_RELU>(v); break;
+    case AQ_ACT_GELU: v = act_value<AQ_ACT_GELU>(v); break;
+    case AQ_ACT_GELU_TANH: v = act_value<AQ_ACT_GELU_TANH>(v); break;
+    case AQ_ACT_SILU: v = act_value<AQ_ACT_SILU>(v); break;
     default: break;
     }
     if (a.residual)
@@ -461,16 +434,14 @@ int few_rows(const GemmArgs& a, cudaStream_t st)
 
 // ------------------------------------------------------------------------------------------------
 // dz = dy act'(z) and the partial sums of db.  A thread owns VEC neighbouring columns, a warp 32 VEC of them, and the
-// 8 warps of a CTA take the rows of its band in turn, four of them in flight per thread; the sums stay in registers
-// until the band ends.  Bound by memory (dy and z in, dz out) once the slope costs few instructions: with erff and
-// expf the gelu form of a bf16 16384 x 11008 layer is bound by issue.
+// 8 warps of a CTA take the rows of its band in turn, two of them in flight per thread; the sums stay in registers
+// until the band ends.  Bound by memory (dy and z in, dz out) once the slope costs few instructions and registers: 16384
+// x 11008 bf16 gelu 739 us element by element with erff and expf, 236 us with 27 instructions per element and 16 warps
+// per SM, 165 us at the copy bandwidth.
 // ------------------------------------------------------------------------------------------------
-constexpr int kBandRowsAtOnce = 4;
-
 template <typename T, int ACT, int VEC>
-__global__ void __launch_bounds__(256) grad_z_kernel(GradZArgs a, int64_t band_rows)
+__global__ void __launch_bounds__(256, VEC > 1 ? 4 : 2) grad_z_kernel(GradZArgs a, int64_t band_rows)
 {
-    constexpr bool FAST = sizeof(T) == 2;
     __shared__ float sh[8][32 * VEC + 4];
     pdl_launch_dependents();
     pdl_wait();
@@ -478,47 +449,90 @@ __global__ void __launch_bounds__(256) grad_z_kernel(GradZArgs a, int64_t band_r
     const int64_t col  = ((int64_t) blockIdx.x * 32 + lane) * VEC;
     const int64_t row0 = (int64_t) blockIdx.y * band_rows;
     const int64_t row1 = row0 + band_rows < a.rows ? row0 + band_rows : a.rows;
-    float db[VEC]      = {};
-    if (col < a.cols)   // VEC divides the number of columns
+    const T* dy = (const T*) a.dy + col;
+    const T* z  = (const T*) a.z + col;
+    T* dz       = (T*) a.dz + col;
+    if constexpr (VEC > 1)
     {
-        const T* dy = (const T*) a.dy + col;
-        const T* z  = (const T*) a.z + col;
-        T* dz       = (T*) a.dz + col;
-        for (int64_t row = row0 + warp; row < row1; row += 8 * kBandRowsAtOnce)
-        {
-            Pack<T, VEC> g[kBandRowsAtOnce], h[kBandRowsAtOnce];
+        constexpr int Q = VEC / 2, AT = 2;
+        f32x2_t db[Q];
 #pragma unroll
-            for (int u = 0; u < kBandRowsAtOnce; ++u)
-                if (row + 8 * u < row1)
+        for (int q = 0; q < Q; ++q)
+            db[q] = pair(0.f, 0.f);
+        auto one = [&](const uint4& g, const uint4& h, int64_t row) {
+            f32x2_t v[Q];
+            expand<T>(g, v);
+            if constexpr (ACT != AQ_ACT_NONE)
+            {
+                f32x2_t zz[Q];
+                expand<T>(h, zz);
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
                 {
-                    g[u] = load_pack<T, VEC>(dy + (row + 8 * u) * a.lddy);
-                    if (ACT != AQ_ACT_NONE)
-                        h[u] = load_pack<T, VEC>(z + (row + 8 * u) * a.ldz);
-                }
-#pragma unroll
-            for (int u = 0; u < kBandRowsAtOnce; ++u)
-                if (row + 8 * u < row1)
-                {
-                    Pack<T, VEC> o;
-#pragma unroll
-                    for (int c = 0; c < VEC; ++c)
+                    if constexpr (sizeof(T) == 2)
+                        v[q] = act_grad2<ACT>(v[q], zz[q]);
+                    else
                     {
-                        float v = to_f32(g[u].v[c]);
-                        if (ACT != AQ_ACT_NONE)
-                            v = act_grad<ACT, FAST>(v, to_f32(h[u].v[c]));
-                        o.v[c] = from_f32<T>(v);
-                        db[c] += v;
+                        float d0, d1, z0, z1;
+                        unpair(v[q], d0, d1);
+                        unpair(zz[q], z0, z1);
+                        v[q] = pair(act_grad<ACT>(d0, z0), act_grad<ACT>(d1, z1));
                     }
-                    if (a.dz)
-                        store_pack<T, VEC>(dz + (row + 8 * u) * a.lddz, o);
                 }
+            }
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                db[q] = add2(db[q], v[q]);
+            if (a.dz)
+                *reinterpret_cast<uint4*>(dz + row * a.lddz) = ACT == AQ_ACT_NONE ? g : compress<T>(v);
+        };
+        if (col < a.cols)   // VEC divides the number of columns
+        {
+            int64_t row = row0 + warp;
+            for (; row + 8 * (AT - 1) < row1; row += 8 * AT)
+            {
+                uint4 g[AT], h[AT];
+#pragma unroll
+                for (int u = 0; u < AT; ++u)
+                {
+                    g[u] = *reinterpret_cast<const uint4*>(dy + (row + 8 * u) * a.lddy);
+                    if (ACT != AQ_ACT_NONE)
+                        h[u] = *reinterpret_cast<const uint4*>(z + (row + 8 * u) * a.ldz);
+                }
+#pragma unroll
+                for (int u = 0; u < AT; ++u)
+                    one(g[u], h[u], row + 8 * u);
+            }
+            for (; row < row1; row += 8)
+                one(*reinterpret_cast<const uint4*>(dy + row * a.lddy),
+                    ACT != AQ_ACT_NONE ? *reinterpret_cast<const uint4*>(z + row * a.ldz) : uint4 {}, row);
         }
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+        {
+            float lo, hi;
+            unpair(db[q], lo, hi);
+            sh[warp][lane * VEC + 2 * q]     = lo;
+            sh[warp][lane * VEC + 2 * q + 1] = hi;
+        }
+    }
+    else
+    {
+        float db = 0.f;
+        if (col < a.cols)
+#pragma unroll 4
+            for (int64_t row = row0 + warp; row < row1; row += 8)
+            {
+                const float g = to_f32(dy[row * a.lddy]);
+                const float v = ACT == AQ_ACT_NONE ? g : act_grad<ACT>(g, to_f32(z[row * a.ldz]));
+                if (a.dz)
+                    dz[row * a.lddz] = from_f32<T>(v);
+                db += v;
+            }
+        sh[warp][lane] = db;
     }
     if (!a.part)
         return;
-#pragma unroll
-    for (int c = 0; c < VEC; ++c)
-        sh[warp][lane * VEC + c] = db[c];
     __syncthreads();
     for (int c = threadIdx.x; c < 32 * VEC; c += 256)
     {
@@ -534,10 +548,13 @@ __global__ void __launch_bounds__(256) grad_z_kernel(GradZArgs a, int64_t band_r
     }
 }
 
-// Bands for `ctas` column tiles: enough CTAs for 8 per SM, at least 64 rows each.
+// Bands for `ctas` column tiles: whole waves of four CTAs per SM as far as that goes, at least 64 rows each.
 int64_t grad_bands(int64_t rows, int64_t ctas)
 {
-    int64_t bands      = (8 * kNumSMs + ctas - 1) / ctas;
+    const int64_t wave = 4 * kNumSMs;
+    int64_t bands      = wave / ctas;
+    if (bands < 8)   // few bands fit into one wave: the loss at its end is smaller with two
+        bands = 2 * wave / ctas;
     const int64_t most = (rows + 63) / 64;
     bands              = bands < most ? bands : most;
     return bands < 1 ? 1 : bands;
@@ -663,8 +680,13 @@ int fold_columns(const float* part, int64_t bands, int64_t stride, int64_t cols,
 
 int64_t grad_z_workspace_bytes(int64_t rows, int64_t cols)
 {
-    // the number of bands falls with the number of column tiles: the widest tiles need the most
-    return grad_bands(rows, (cols + 255) / 256) * cols * (int64_t) sizeof(float);
+    int64_t bands = 1;
+    for (int64_t width : {32, 128, 256})   // of a CTA, by type and alignment
+    {
+        const int64_t n = grad_bands(rows, (cols + width - 1) / width);
+        bands           = n > bands ? n : bands;
+    }
+    return bands * cols * (int64_t) sizeof(float);
 }
 
 int grad_z(const GradZArgs& a, cudaStream_t st)

@@ -38,31 +38,22 @@ struct TcArgs
 constexpr int kBlockK   = 64;   // one 128-byte row of the swizzle
 constexpr int kPairWarps = 8;   // epilogue warps of pair_kernel
 
+template <int ACT, int N>
+__device__ __forceinline__ void activate_as(float (&v)[N])
+{
+#pragma unroll
+    for (int c = 0; c < N; c += 2)
+        unpair(act_value2<ACT>(pair(v[c], v[c + 1])), v[c], v[c + 1]);
+}
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], int act)
 {
     switch (act)
     {
-    case AQ_ACT_RELU:
-#pragma unroll
-        for (int c = 0; c < N; ++c)
-            v[c] = act_value<AQ_ACT_RELU, true>(v[c]);
-        break;
-    case AQ_ACT_GELU:
-#pragma unroll
-        for (int c = 0; c < N; ++c)
-            v[c] = act_value<AQ_ACT_GELU, true>(v[c]);
-        break;
-    case AQ_ACT_GELU_TANH:
-#pragma unroll
-        for (int c = 0; c < N; ++c)
-            v[c] = act_value<AQ_ACT_GELU_TANH, true>(v[c]);
-        break;
-    case AQ_ACT_SILU:
-#pragma unroll
-        for (int c = 0; c < N; ++c)
-            v[c] = act_value<AQ_ACT_SILU, true>(v[c]);
-        break;
+    case AQ_ACT_RELU: activate_as<AQ_ACT_RELU>(v); break;
+    case AQ_ACT_GELU: activate_as<AQ_ACT_GELU>(v); break;
+    case AQ_ACT_GELU_TANH: activate_as<AQ_ACT_GELU_TANH>(v); break;
+    case AQ_ACT_SILU: activate_as<AQ_ACT_SILU>(v); break;
     default: break;
     }
 }

@@ -348,7 +348,11 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
                 float acc[32];
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
-                    acc[c] = poison ? __int_as_float(0x7fffffff) : __uint_as_float(raw[c]);
+                    acc[c] = __uint_as_float(raw[c]);
+                if (poison)
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        acc[c] = __int_as_float(0x7fffffff);
                 const int64_t j = col0 + c0;
                 if (p.vec == 16)
                 {

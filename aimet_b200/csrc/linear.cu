@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
             z += tc::ld_cluster(tc::map_to(base + e * 4, r));
         finish(z, i0 + e / TILE, j0 + e % TILE);
     }
-    tc::cluster_sync();   // nobody leaves while its partial tile may be read
+    tc::cluster_meet();   // nobody leaves while its partial tile may be read
 }
 
 template <int TILE, bool AK, bool BK>

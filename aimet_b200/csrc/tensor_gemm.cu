@@ -32,7 +32,7 @@ struct TcArgs
     uint32_t idesc;
     int a_kmajor, b_kmajor;
     int tiles_i, tiles_j;
-    int vec;             // pair_kernel: elements per access of out / z / residual: 16, 8, or 0 (through shared memory)
+    int vec;             // elements per access that out, z and residual allow: 16, 8, or 0
 };
 
 constexpr int kBlockK   = 64;   // one 128-byte row of the swizzle
@@ -58,39 +58,40 @@ __device__ __forceinline__ void activate(float (&v)[N], int act)
     }
 }
 
-// N (8 or 16) 16-bit elements as one access of 16 or 32 bytes
-template <typename T, int N>
-__device__ __forceinline__ void load_wide(const T* p, T (&v)[N])
+// 16 neighbouring elements as float32 lanes.  `wide`: one access of 32 bytes, else two of 16, of which the second only if
+// `all` 16 exist.
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, f32x2_t (&f)[8], bool wide, bool all)
 {
-    uint32_t w[N / 2];
-    if constexpr (N == 16)
+    uint4 lo, hi = make_uint4(0, 0, 0, 0);
+    if (wide)
         asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                     : "l"(p)
-                     : "memory");
+                     : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
+                     : "l"(p));
     else
-        asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "l"(p)
-                     : "memory");
-    memcpy(v, w, sizeof w);
+    {
+        lo = *reinterpret_cast<const uint4*>(p);
+        if (all)
+            hi = *reinterpret_cast<const uint4*>(p + 8);
+    }
+    expand<T>(lo, reinterpret_cast<f32x2_t(&)[4]>(f[0]));
+    expand<T>(hi, reinterpret_cast<f32x2_t(&)[4]>(f[4]));
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_wide(T* p, const float (&f)[N])
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const f32x2_t (&f)[8], bool wide, bool all)
 {
-    T v[N];
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-        v[c] = from_f32<T>(f[c]);
-    uint32_t w[N / 2];
-    memcpy(w, v, sizeof w);
-    if constexpr (N == 16)
-        asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(p)
+    const uint4 lo = compress<T>(reinterpret_cast<const f32x2_t(&)[4]>(f[0]));
+    const uint4 hi = compress<T>(reinterpret_cast<const f32x2_t(&)[4]>(f[4]));
+    if (wide)
+        asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w),
+                     "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w), "l"(p)
                      : "memory");
     else
-        asm volatile("st.global.v4.b32 [%4], {%0, %1, %2, %3};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "l"(p)
-                     : "memory");
+    {
+        *reinterpret_cast<uint4*>(p) = lo;
+        if (all)
+            *reinterpret_cast<uint4*>(p + 8) = hi;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -116,40 +117,44 @@ __device__ __forceinline__ void tile_at(int t, int tiles_i, int tiles_j, int& ti
     ti             = band * 8 + in_band - tj * h;
 }
 
-// One epilogue chunk of N columns for a thread that holds one row of them.
-template <typename T, int N>
-__device__ __forceinline__ void row_chunk(const TcArgs& p, const float* acc, int64_t i, int64_t j, bool row_ok)
+// 16 columns from j of row i, which the thread holds; rows start on 16-byte boundaries everywhere (32 when `wide`).
+template <typename T, int ACT>
+__device__ __forceinline__ void row_chunk(const TcArgs& p, f32x2_t (&v)[8], int64_t i, int64_t j, bool wide)
 {
-    if (j >= p.cols || !row_ok)
-        return;
-    float f[N];
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-        f[c] = acc[c];
+    const bool all = j + 16 <= p.cols;   // the number of columns is a multiple of 8
+    f32x2_t r[8];
+    if (p.residual)
+        load16<T>((const T*) p.residual + i * p.ldr + j, r, wide, all);
     if (p.bias)
     {
+        const T* b = (const T*) p.bias + j;
 #pragma unroll
-        for (int c = 0; c < N; ++c)
-            f[c] += to_f32(((const T*) p.bias)[j + c]);
+        for (int q = 0; q < 8; ++q)
+            if (q < 4 || all)
+                v[q] = add2(v[q], pair(to_f32(b[2 * q]), to_f32(b[2 * q + 1])));
     }
     if (p.z)
-        store_wide<T, N>((T*) p.z + i * p.ldz + j, f);
-    activate<N>(f, p.act);
+        store16<T>((T*) p.z + i * p.ldz + j, v, wide, all);
+    if constexpr (ACT != AQ_ACT_NONE)
+    {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            v[q] = act_value2<ACT>(v[q]);
+    }
     if (p.residual)
     {
-        T r[N];
-        load_wide<T, N>((const T*) p.residual + i * p.ldr + j, r);
 #pragma unroll
-        for (int c = 0; c < N; ++c)
-            f[c] += to_f32(r[c]);
+        for (int q = 0; q < 8; ++q)
+            v[q] = add2(v[q], r[q]);
     }
-    store_wide<T, N>((T*) p.out + i * p.ldo + j, f);
+    store16<T>((T*) p.out + i * p.ldo + j, v, wide, all);
 }
 
 // One epilogue chunk of N rows (the first `most` of them exist) for a thread that holds one column of them; z is acc.
+// ACT = -1: the activation comes with the arguments.
 // The residuals are fetched together: one at a time their latency is what the epilogue waits for (a 777 x 1537 result:
 // 30 us against 8 us).
-template <typename T, int N>
+template <typename T, int N, int ACT = -1>
 __device__ __forceinline__ void column_chunk(const TcArgs& p, float (&acc)[N], int64_t i, int most, int64_t j)
 {
     T r[N];
@@ -157,29 +162,55 @@ __device__ __forceinline__ void column_chunk(const TcArgs& p, float (&acc)[N], i
     {
         const T* src = (const T*) p.residual + i * p.ldr + j;
 #pragma unroll
-        for (int u = 0; u < N; ++u)
+        for (int u = 0; u < N; ++u, src += p.ldr)
             if (u < most)
-                r[u] = src[u * p.ldr];
+                r[u] = *src;
     }
     if (p.z)
     {
         T* dst = (T*) p.z + i * p.ldz + j;
 #pragma unroll
-        for (int u = 0; u < N; ++u)
+        for (int u = 0; u < N; ++u, dst += p.ldz)
             if (u < most)
-                dst[u * p.ldz] = from_f32<T>(acc[u]);
+                *dst = from_f32<T>(acc[u]);
     }
-    activate<N>(acc, p.act);
+    if constexpr (ACT < 0)
+        activate<N>(acc, p.act);
+    else if constexpr (ACT != AQ_ACT_NONE)
+        activate_as<ACT, N>(acc);
     T* dst = (T*) p.out + i * p.ldo + j;
 #pragma unroll
-    for (int u = 0; u < N; ++u)
+    for (int u = 0; u < N; ++u, dst += p.ldo)
         if (u < most)
-            dst[u * p.ldo] = from_f32<T>(p.residual ? acc[u] + to_f32(r[u]) : acc[u]);
+            *dst = from_f32<T>(p.residual ? acc[u] + to_f32(r[u]) : acc[u]);
 }
 
-template <typename T, int BN>
+// A warp's 32 x 32 patch of z without bias in shared memory, [row][33], to rows that no wide access fits.  Not inlined: its
+// addresses would push the registers of the other path out to memory.
+template <typename T, int ACT>
+__device__ __noinline__ void write_patch(const TcArgs& p, const float* patch, int64_t row0, int64_t j)
+{
+    const int lane = threadIdx.x & 31;
+    j += lane;
+    if (j >= p.cols)
+        return;
+    const float bias = p.bias ? to_f32(((const T*) p.bias)[j]) : 0.f;
+    const int most   = p.rows - row0 < 32 ? (int) (p.rows - row0) : 32;
+#pragma unroll 1
+    for (int r = 0; r < most; r += 16)
+    {
+        float v[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            v[u] = patch[(r + u) * 33 + lane] + bias;
+        column_chunk<T, 16, ACT>(p, v, row0 + r, most - r, j);
+    }
+}
+
+template <typename T, int BN, int ACT>
 __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
-    pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const TcArgs p)
+    pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ TcArgs p)
 {
     using S = PairShape<BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -223,13 +254,14 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
     const int tiles = p.tiles_i * p.tiles_j;
     const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
 
-    if (warp == 0 && lane == 0)
+    if (warp == 0)
     {
         // ---- producer: this CTA's 128 rows of A and BN / 2 rows of B per stage, reported to the leader's barrier ----
         int s = 0;
         uint32_t phase = 0;
         bool ok        = true;
         int used       = 0;
+        const uint32_t full0 = map_to(full, 0);
         for (int t = first; t < tiles && ok; t += stride)
         {
             int ti, tj;
@@ -237,29 +269,33 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
             const int i0 = ti * 256 + (int) rank * 128, j0 = tj * BN + (int) rank * (BN / 2);
             for (int kb = 0; kb < p.k_blocks; ++kb)
             {
-                ok = mbar_wait(empty + 8 * s, phase ^ 1u, stuck);
+                ok = mbar_wait_warp(empty + 8 * s, phase ^ 1u, stuck);
                 if (!ok)
                     break;
-                if (rank == 0)
-                    mbar_expect(full + 8 * s, 2 * S::kStageBytes);
-                const uint32_t bar = map_to(full + 8 * s, 0);
-                const uint32_t sa = base + s * S::kStageBytes, sb = sa + 128 * 128;
-                const int k0 = kb * kBlockK;
-                if (p.a_kmajor)
-                    tma_load_pair(sa, &map_a, k0, i0, bar);
-                else
+                if (elect_one())
                 {
-                    tma_load_pair(sa, &map_a, i0, k0, bar);
-                    tma_load_pair(sa + 8192, &map_a, i0 + 64, k0, bar);
+                    if (rank == 0)
+                        mbar_expect(full + 8 * s, 2 * S::kStageBytes);
+                    const uint32_t bar = full0 + 8 * s;
+                    const uint32_t sa = base + s * S::kStageBytes, sb = sa + 128 * 128;
+                    const int k0 = kb * kBlockK;
+                    if (p.a_kmajor)
+                        tma_load_pair(sa, &map_a, k0, i0, bar);
+                    else
+                    {
+                        tma_load_pair(sa, &map_a, i0, k0, bar);
+                        tma_load_pair(sa + 8192, &map_a, i0 + 64, k0, bar);
+                    }
+                    if (p.b_kmajor)
+                        tma_load_pair(sb, &map_b, k0, j0, bar);
+                    else
+                    {
+                        tma_load_pair(sb, &map_b, j0, k0, bar);
+                        if constexpr (BN == 256)
+                            tma_load_pair(sb + 8192, &map_b, j0 + 64, k0, bar);
+                    }
                 }
-                if (p.b_kmajor)
-                    tma_load_pair(sb, &map_b, k0, j0, bar);
-                else
-                {
-                    tma_load_pair(sb, &map_b, j0, k0, bar);
-                    if constexpr (BN == 256)
-                        tma_load_pair(sb + 8192, &map_b, j0 + 64, k0, bar);
-                }
+                __syncwarp();
                 used = used < S::kStages ? used + 1 : used;
                 if (++s == S::kStages)
                 {
@@ -271,7 +307,7 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
         // every stage in use is handed back before the CTA may end: the releases arrive in this CTA's memory
         for (int u = 0; u < used && ok; ++u)
         {
-            ok = mbar_wait(empty + 8 * s, phase ^ 1u, stuck);
+            ok = mbar_wait_warp(empty + 8 * s, phase ^ 1u, stuck);
             if (++s == S::kStages)
             {
                 s = 0;
@@ -279,40 +315,43 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
             }
         }
     }
-    else if (warp == 1 && lane == 0 && rank == 0)
+    else if (warp == 1 && rank == 0)
     {
-        // ---- one thread of the leader issues the matrix instructions of both SMs ----
+        // ---- one lane of the leader issues the matrix instructions of both SMs ----
         int s = 0;
         uint32_t phase = 0;
         bool ok        = true;
         int n          = 0;
         const uint32_t step_a = operand_step(p.a_kmajor), step_b = operand_step(p.b_kmajor);
+        const uint64_t desc_a = operand_desc(base, p.a_kmajor), desc_b = operand_desc(base + 128 * 128, p.b_kmajor);
         for (int t = first; t < tiles && ok; t += stride, ++n)
         {
             const int buf    = n & 1;
             const uint32_t d = tmem + buf * BN;
-            ok               = mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1u, stuck);
+            ok               = mbar_wait_warp(tempty + 8 * buf, ((n >> 1) & 1) ^ 1u, stuck);
             tmem_fence_after();
             for (int kb = 0; kb < p.k_blocks && ok; ++kb)
             {
-                ok = mbar_wait(full + 8 * s, phase, stuck);
+                ok = mbar_wait_warp(full + 8 * s, phase, stuck);
                 if (!ok)
                     break;
-                tmem_fence_after();
-                const uint32_t sa = base + s * S::kStageBytes;
-                const uint64_t da = operand_desc(sa, p.a_kmajor), db = operand_desc(sa + 128 * 128, p.b_kmajor);
+                if (elect_one())
+                {
+                    const uint64_t da = desc_a + s * (S::kStageBytes >> 4), db = desc_b + s * (S::kStageBytes >> 4);
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    mma<2>(d, da + u * step_a, db + u * step_b, p.idesc, kb > 0 || u > 0);
-                mma_commit_pair(empty + 8 * s, 3);
+                    for (int u = 0; u < 4; ++u)
+                        mma<2>(d, da + u * step_a, db + u * step_b, p.idesc, kb > 0 || u > 0);
+                    mma_commit_pair(empty + 8 * s, 3);
+                    if (kb + 1 == p.k_blocks)
+                        mma_commit_pair(tfull + 8 * buf, 3);
+                }
+                __syncwarp();
                 if (++s == S::kStages)
                 {
                     s = 0;
                     phase ^= 1u;
                 }
             }
-            if (ok)
-                mma_commit_pair(tfull + 8 * buf, 3);
         }
     }
     else if (warp >= 4)
@@ -327,11 +366,11 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
             int ti, tj;
             tile_at(t, p.tiles_i, p.tiles_j, ti, tj);
             const int buf     = n & 1;
-            const bool ok     = mbar_wait(tfull + 8 * buf, (n >> 1) & 1, stuck);
-            const bool poison = __any_sync(0xffffffffu, !ok);
+            const bool poison = !mbar_wait_warp(tfull + 8 * buf, (n >> 1) & 1, stuck);
             tmem_fence_after();
             const int64_t row0 = (int64_t) ti * 256 + rank * 128 + quarter * 32;
             const int64_t col0 = (int64_t) tj * BN + half * (BN / 2);
+#pragma unroll 1
             for (int c0 = 0; c0 < BN / 2; c0 += 32)
             {
                 uint32_t raw[32];
@@ -345,27 +384,24 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
                     if (lane == 0)
                         mbar_arrive_cluster(release0 + 8 * buf);
                 }
-                float acc[32];
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                    acc[c] = __uint_as_float(raw[c]);
                 if (poison)
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
-                        acc[c] = __int_as_float(0x7fffffff);
+                        raw[c] = 0x7fffffff;
                 const int64_t j = col0 + c0;
-                if (p.vec == 16)
-                {
-                    const int64_t i = row0 + lane;
-                    row_chunk<T, 16>(p, acc, i, j, i < p.rows);
-                    row_chunk<T, 16>(p, acc + 16, i, j + 16, i < p.rows);
-                }
-                else if (p.vec == 8)
+                if (p.vec)
                 {
                     const int64_t i = row0 + lane;
 #pragma unroll
-                    for (int g = 0; g < 32; g += 8)
-                        row_chunk<T, 8>(p, acc + g, i, j + g, i < p.rows);
+                    for (int g = 0; g < 32; g += 16)
+                        if (i < p.rows && j + g < p.cols)
+                        {
+                            f32x2_t v[8];
+#pragma unroll
+                            for (int q = 0; q < 8; ++q)
+                                v[q] = pair(__uint_as_float(raw[g + 2 * q]), __uint_as_float(raw[g + 2 * q + 1]));
+                            row_chunk<T, ACT>(p, v, i, j + g, p.vec == 16);
+                        }
                 }
                 else
                 {
@@ -373,23 +409,9 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
                     __syncwarp();
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
-                        patch[lane * 33 + c] = acc[c];
+                        patch[lane * 33 + c] = __uint_as_float(raw[c]);
                     __syncwarp();
-                    const int64_t jj = j + lane;
-                    if (jj < p.cols)
-                    {
-                        const float bias = p.bias ? to_f32(((const T*) p.bias)[jj]) : 0.f;
-                        const int most   = p.rows - row0 < 32 ? (int) (p.rows - row0) : 32;
-#pragma unroll 1
-                        for (int r = 0; r < most; r += 16)
-                        {
-                            float v[16];
-#pragma unroll
-                            for (int u = 0; u < 16; ++u)
-                                v[u] = patch[(r + u) * 33 + lane] + bias;
-                            column_chunk<T, 16>(p, v, row0 + r, most - r, jj);
-                        }
-                    }
+                    write_patch<T, ACT>(p, patch, row0, j);
                 }
             }
         }
@@ -398,7 +420,7 @@ __global__ void __launch_bounds__(128 + 32 * kPairWarps, 1)
     stuck_exit(stuck, &g_stuck);
     tmem_fence_before();
     __syncthreads();
-    cluster_sync();
+    cluster_meet();
     tmem_fence_after();
     if (warp == 2)
         tmem_free<2>(tmem, 2 * BN);
@@ -419,9 +441,59 @@ struct SlimShape
     static_assert(BN * 128 * 4 <= kBars, "the partial results of a CTA take the place of its operand tiles");
 };
 
+// Four results of row i from column j.  With p.vec every row starts on a 16-byte boundary and the number of columns is a
+// multiple of 8.
+template <typename T>
+__device__ __forceinline__ void quad(const TcArgs& p, const float4& z, int64_t i, int64_t j)
+{
+    float v[4] = {z.x, z.y, z.z, z.w};
+    if (p.vec)
+    {
+        if (j >= p.cols)
+            return;
+        auto store = [&](T* dst) {
+            Pack<T, 4> o;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                o.v[u] = from_f32<T>(v[u]);
+            store_pack<T, 4>(dst, o);
+        };
+        Pack<T, 4> r;
+        if (p.residual)
+            r = load_pack<T, 4>((const T*) p.residual + i * p.ldr + j);
+        if (p.z)
+            store((T*) p.z + i * p.ldz + j);
+        activate<4>(v, p.act);
+        if (p.residual)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                v[u] += to_f32(r.v[u]);
+        store((T*) p.out + i * p.ldo + j);
+    }
+    else
+    {
+        T r[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (j + u < p.cols)
+            {
+                if (p.residual)
+                    r[u] = ((const T*) p.residual)[i * p.ldr + j + u];
+                if (p.z)
+                    ((T*) p.z)[i * p.ldz + j + u] = from_f32<T>(v[u]);
+            }
+        activate<4>(v, p.act);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (j + u < p.cols)
+                ((T*) p.out)[i * p.ldo + j + u] = from_f32<T>(p.residual ? v[u] + to_f32(r[u]) : v[u]);
+    }
+}
+
 template <typename T, int BN>
 __global__ void __launch_bounds__(192, 2)
-    slim_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const TcArgs p)
+    slim_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ TcArgs p)
 {
     using S = SlimShape<BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -463,32 +535,36 @@ __global__ void __launch_bounds__(192, 2)
     const int i0 = ti * BN, j0 = tj * 128;
     const int kb0 = (int) ((int64_t) p.k_blocks * rank / splits), kb1 = (int) ((int64_t) p.k_blocks * (rank + 1) / splits);
 
-    if (warp == 0 && lane == 0)
+    if (warp == 0)
     {
         int s = 0;
         uint32_t phase = 0;
         for (int kb = kb0; kb < kb1; ++kb)
         {
-            if (!mbar_wait(empty + 8 * s, phase ^ 1u, stuck))
+            if (!mbar_wait_warp(empty + 8 * s, phase ^ 1u, stuck))
                 break;
-            mbar_expect(full + 8 * s, S::kStageBytes);
-            const uint32_t sf = base + s * S::kStageBytes, sr = sf + 128 * 128;
-            const int k0 = kb * kBlockK;
-            if (p.b_kmajor)
-                tma_load(sf, &map_b, k0, j0, full + 8 * s);
-            else
+            if (elect_one())
             {
-                tma_load(sf, &map_b, j0, k0, full + 8 * s);
-                tma_load(sf + 8192, &map_b, j0 + 64, k0, full + 8 * s);
-            }
-            if (p.a_kmajor)
-                tma_load(sr, &map_a, k0, i0, full + 8 * s);
-            else
-            {
+                mbar_expect(full + 8 * s, S::kStageBytes);
+                const uint32_t sf = base + s * S::kStageBytes, sr = sf + 128 * 128;
+                const int k0 = kb * kBlockK;
+                if (p.b_kmajor)
+                    tma_load(sf, &map_b, k0, j0, full + 8 * s);
+                else
+                {
+                    tma_load(sf, &map_b, j0, k0, full + 8 * s);
+                    tma_load(sf + 8192, &map_b, j0 + 64, k0, full + 8 * s);
+                }
+                if (p.a_kmajor)
+                    tma_load(sr, &map_a, k0, i0, full + 8 * s);
+                else
+                {
 #pragma unroll
-                for (int u = 0; u < BN / 64; ++u)   // column operands have BN of 64 or more
-                    tma_load(sr + 8192 * u, &map_a, i0 + 64 * u, k0, full + 8 * s);
+                    for (int u = 0; u < BN / 64; ++u)   // column operands have BN of 64 or more
+                        tma_load(sr + 8192 * u, &map_a, i0 + 64 * u, k0, full + 8 * s);
+                }
             }
+            __syncwarp();
             if (++s == S::kStages)
             {
                 s = 0;
@@ -496,32 +572,33 @@ __global__ void __launch_bounds__(192, 2)
             }
         }
     }
-    else if (warp == 1 && lane == 0)
+    else if (warp == 1)
     {
         int s = 0;
         uint32_t phase = 0;
-        bool ok        = true;
         const uint32_t step_f = operand_step(p.b_kmajor), step_r = operand_step(p.a_kmajor);
+        const uint64_t desc_f = operand_desc(base, p.b_kmajor), desc_r = operand_desc(base + 128 * 128, p.a_kmajor);
         for (int kb = kb0; kb < kb1; ++kb)
         {
-            ok = mbar_wait(full + 8 * s, phase, stuck);
-            if (!ok)
+            if (!mbar_wait_warp(full + 8 * s, phase, stuck))
                 break;
-            tmem_fence_after();
-            const uint32_t sf = base + s * S::kStageBytes;
-            const uint64_t df = operand_desc(sf, p.b_kmajor), dr = operand_desc(sf + 128 * 128, p.a_kmajor);
+            if (elect_one())
+            {
+                const uint64_t df = desc_f + s * (S::kStageBytes >> 4), dr = desc_r + s * (S::kStageBytes >> 4);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                mma<1>(tmem, df + u * step_f, dr + u * step_r, p.idesc, kb > kb0 || u > 0);
-            mma_commit(empty + 8 * s);
+                for (int u = 0; u < 4; ++u)
+                    mma<1>(tmem, df + u * step_f, dr + u * step_r, p.idesc, kb > kb0 || u > 0);
+                mma_commit(empty + 8 * s);
+                if (kb + 1 == kb1)
+                    mma_commit(tfull);
+            }
+            __syncwarp();
             if (++s == S::kStages)
             {
                 s = 0;
                 phase ^= 1u;
             }
         }
-        if (ok)
-            mma_commit(tfull);
     }
     __syncwarp();
     float* part = reinterpret_cast<float*>(smem_raw + (base - smem_addr(smem_raw)));   // [BN][128]
@@ -531,9 +608,9 @@ __global__ void __launch_bounds__(192, 2)
     bool poison       = false;
     if (warp >= 2)
     {
-        if (p.bias && j < p.cols)
+        if (p.bias && splits == 1 && j < p.cols)
             bias = to_f32(((const T*) p.bias)[j]);
-        poison = __any_sync(0xffffffffu, !mbar_wait(tfull, 0, stuck));
+        poison = !mbar_wait_warp(tfull, 0, stuck);
         tmem_fence_after();
     }
     const float bad = __int_as_float(0x7fffffff);
@@ -566,34 +643,58 @@ __global__ void __launch_bounds__(192, 2)
     {
         __syncwarp();
         cluster_sync();
-        if (warp >= 2 && j < p.cols)
+        if (warp >= 2)
         {
+            // every CTA finishes its share of the rows: a warp takes a row, a lane four columns of it, four rows at a time
             const int c0 = rows * (int) rank / (int) splits, c1 = rows * (int) (rank + 1) / (int) splits;
-            const uint32_t mine = smem_addr(part) + f * 4;
-            constexpr int AT = BN < 8 * 8 ? 4 : 8;   // rows joined at a time
-#pragma unroll 1
-            for (int c = c0; c < c1; c += AT)
+            const int64_t jq = (int64_t) j0 + lane * 4;
+            const uint32_t from = smem_addr(part) + lane * 16;
+            float4 b4 = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p.bias)
             {
-                float v[AT] = {};
-                for (uint32_t r = 0; r < splits; ++r)   // always in this order: the same bits on every run
+                const T* b = (const T*) p.bias + jq;
+                b4         = make_float4(jq < p.cols ? to_f32(b[0]) : 0.f, jq + 1 < p.cols ? to_f32(b[1]) : 0.f,
+                                         jq + 2 < p.cols ? to_f32(b[2]) : 0.f, jq + 3 < p.cols ? to_f32(b[3]) : 0.f);
+            }
+#pragma unroll 1
+            for (int c = c0 + warp - 2; c < c1; c += 16)
+            {
+                float4 v[4] = {b4, b4, b4, b4};
+#pragma unroll 1
+                for (uint32_t r = 0; r < splits; r += 4)
                 {
-                    const uint32_t from = map_to(mine + c * 512, r);
-                    float w[AT];
+                    float4 w[4][4];   // [part][row], all on their way together
 #pragma unroll
-                    for (int u = 0; u < AT; ++u)
-                        w[u] = c + u < c1 ? ld_cluster(from + u * 512) : 0.f;
+                    for (int q = 0; q < 4; ++q)
+                        if (r + q < splits)
+                        {
+                            const uint32_t at = map_to(from + c * 512, r + q);
 #pragma unroll
-                    for (int u = 0; u < AT; ++u)
-                        v[u] += w[u];
+                            for (int u = 0; u < 4; ++u)
+                                if (c + 4 * u < c1)
+                                    w[q][u] = ld_cluster4(at + 4 * u * 512);
+                        }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)   // always in this order: the same bits on every run
+                        if (r + q < splits)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+                                if (c + 4 * u < c1)
+                                {
+                                    v[u].x += w[q][u].x;
+                                    v[u].y += w[q][u].y;
+                                    v[u].z += w[q][u].z;
+                                    v[u].w += w[q][u].w;
+                                }
                 }
 #pragma unroll
-                for (int u = 0; u < AT; ++u)
-                    v[u] += bias;
-                column_chunk<T, AT>(p, v, i0 + c, c1 - c, j);
+                for (int u = 0; u < 4; ++u)
+                    if (c + 4 * u < c1)
+                        quad<T>(p, v[u], i0 + c + 4 * u, jq);
             }
         }
         __syncwarp();
-        cluster_sync();   // nobody leaves while its partial results may be read
+        cluster_meet();   // nobody leaves while its partial results may be read
     }
     stuck_exit(stuck, &g_stuck);
     tmem_fence_before();
@@ -635,7 +736,7 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int64_
     const cuuint32_t strides[2] = {1, 1};
     const CUresult r =
         fn(map, dtype == AQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
-           dims, pitch, box, strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           dims, pitch, box, strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? AQ_OK : AQ_ERR_INVALID_ARG;
 }
@@ -707,7 +808,10 @@ int run_pair(const GemmArgs& a, cudaStream_t st)
     if (tiles > 0x3fffffff)
         return AQ_ERR_TOO_LARGE;
     const int64_t pairs = tiles < kNumSMs / 2 ? tiles : kNumSMs / 2;
-    return launch(pair_kernel<T, BN>, 2 * pairs, 2, 128 + 32 * kPairWarps, PairShape<BN>::kSmem, st, ma, mb, p);
+    return with_activation(a.act, [&](auto act) {
+        return launch(pair_kernel<T, BN, decltype(act)::value>, 2 * pairs, 2, 128 + 32 * kPairWarps, PairShape<BN>::kSmem, st, ma,
+                      mb, p);
+    });
 }
 
 template <typename T, int BN>
@@ -722,6 +826,7 @@ int run_slim(const GemmArgs& a, int splits, cudaStream_t st)
     TcArgs p  = tc_args(a);
     p.tiles_i = (int) ((a.rows + BN - 1) / BN);
     p.tiles_j = (int) ((a.cols + 127) / 128);
+    p.vec     = wide_access(a);
     // the columns' operand is the instruction's A
     p.idesc = instruction_desc(a.dtype == AQ_BF16, a.b_kmajor, a.a_kmajor, 128, BN);
     return launch(slim_kernel<T, BN>, (int64_t) p.tiles_i * p.tiles_j * splits, splits, 192, SlimShape<BN>::kSmem, st, ma, mb, p);
@@ -761,22 +866,27 @@ int resident_clusters(int splits)
     return n;
 }
 
-// CTAs of a cluster that share the depth, and the blocks of 64 k that the kernel's longest chain of CTAs then walks: a
-// second wave costs more than a larger cluster gains (24 x 11008 -> 4096: 32 tiles by eight CTAs are two waves and 37 us,
-// by seven one).  Filling the pipeline and joining the parts is worth about 8 blocks.
+// How many CTAs share the depth.  `cost` is what the kernel's longest chain of CTAs takes, in cycles: 64 k of a tile cost 290
+// of them (BN 16 to 64) or 560 (BN 128; both operands then keep the shared memory as busy as the tensor cores could make
+// it) with one CTA on the SM, twice that with two, joining the parts 5000 (BN 128: 9000), the rest 3500.  A second wave of
+// clusters costs more than a larger cluster gains (24 x 11008 -> 4096: 32 tiles by eight CTAs are two waves and 37 us, by
+// seven one and 22).
 template <typename T, int BN>
-int64_t slim_plan(int64_t tiles, int64_t k_blocks, int& splits)
+int slim_plan(int64_t tiles, int64_t k_blocks, int64_t& cost)
 {
-    int64_t best = INT64_MAX;
-    splits       = 1;
+    const int64_t block = BN == 128 ? 560 : 290, join = BN == 128 ? 9000 : 5000;
+    int best = 1;
+    cost     = INT64_MAX;
     for (int s = 1; s <= 8 && (s == 1 || k_blocks >= 4 * s); ++s)
     {
-        const int64_t room = resident_clusters<T, BN>(s);
-        const int64_t cost = (tiles + room - 1) / room * ((k_blocks + s - 1) / s + 8);
-        if (cost < best)
+        const int64_t room  = resident_clusters<T, BN>(s);
+        const int64_t waves = (tiles + room - 1) / room;
+        const int64_t per   = tiles * s > kNumSMs ? 2 * block : block;
+        const int64_t c     = waves * ((k_blocks + s - 1) / s) * per + (s > 1 ? join : 0) + 3500;
+        if (c < cost)
         {
-            best   = cost;
-            splits = s;
+            cost = c;
+            best = s;
         }
     }
     return best;
@@ -785,32 +895,25 @@ int64_t slim_plan(int64_t tiles, int64_t k_blocks, int& splits)
 template <typename T>
 int tensor_gemm_t(const GemmArgs& a, cudaStream_t st)
 {
-    const int64_t kb    = (a.depth + kBlockK - 1) / kBlockK;
-    auto slim_tiles     = [&](int bn) { return (a.rows + bn - 1) / bn * ((a.cols + 127) / 128); };
-    int splits          = 1;
+    const int64_t kb = (a.depth + kBlockK - 1) / kBlockK;
+    auto slim_tiles  = [&](int bn) { return (a.rows + bn - 1) / bn * ((a.cols + 127) / 128); };
+    int64_t slim     = 0;
     if (a.rows <= 64 && a.a_kmajor)
     {
         if (a.rows <= 16)
-        {
-            slim_plan<T, 16>(slim_tiles(16), kb, splits);
-            return run_slim<T, 16>(a, splits, st);
-        }
+            return run_slim<T, 16>(a, slim_plan<T, 16>(slim_tiles(16), kb, slim), st);
         if (a.rows <= 32)
-        {
-            slim_plan<T, 32>(slim_tiles(32), kb, splits);
-            return run_slim<T, 32>(a, splits, st);
-        }
-        slim_plan<T, 64>(slim_tiles(64), kb, splits);
-        return run_slim<T, 64>(a, splits, st);
+            return run_slim<T, 32>(a, slim_plan<T, 32>(slim_tiles(32), kb, slim), st);
+        return run_slim<T, 64>(a, slim_plan<T, 64>(slim_tiles(64), kb, slim), st);
     }
-    // Estimated cycles: a stage of pair_kernel costs 512 (BN 256) or 384 (BN 128), one of slim_kernel 1024 with two CTAs on
-    // the SM; the other term of pair_kernel stands for filling the pipeline and the epilogue.
+    // The same estimate for pair_kernel: 512 cycles for 64 k of a 256 x 256 tile (the tensor cores' own rate), 400 of a
+    // 256 x 128 one (issue and handshakes).  512 x 4096 -> 4096: 23.8 and 20.5 us, slim_kernel 22.9.
     auto waves = [](int64_t n, int64_t slots) { return (n + slots - 1) / slots; };
     const int64_t rt = (a.rows + 255) / 256;
-    const int64_t p256 = waves(rt * ((a.cols + 255) / 256), kNumSMs / 2) * (kb * 512 + 1500);
-    const int64_t p128 = waves(rt * ((a.cols + 127) / 128), kNumSMs / 2) * (kb * 384 + 1000);
-    const int64_t s128 = slim_plan<T, 128>(slim_tiles(128), kb, splits) * 1024;
-    if (s128 < p256 && s128 < p128)
+    const int64_t p256 = waves(rt * ((a.cols + 255) / 256), kNumSMs / 2) * kb * 512 + 4500;
+    const int64_t p128 = waves(rt * ((a.cols + 127) / 128), kNumSMs / 2) * kb * 400 + 4000;
+    const int splits   = slim_plan<T, 128>(slim_tiles(128), kb, slim);
+    if (slim < p256 && slim < p128)
         return run_slim<T, 128>(a, splits, st);
     return p256 <= p128 ? run_pair<T, 256>(a, st) : run_pair<T, 128>(a, st);
 }

@@ -16,7 +16,6 @@ AQ_OK = 0
 AQ_F32, AQ_F16, AQ_BF16 = 0, 1, 2
 AQ_V2_OUT_QDQ, AQ_V2_OUT_CODES = 0, 1
 AQ_ACT_NONE, AQ_ACT_RELU, AQ_ACT_GELU, AQ_ACT_GELU_TANH, AQ_ACT_SILU = 0, 1, 2, 3, 4
-AQ_LINEAR_FEW_ROWS = 8
 AQ_PDF_SIZE = 512
 AQ_TFE_HIST_MANY = 16
 AQ_V2HIST_MAX_BINS = 4096

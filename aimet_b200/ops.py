@@ -264,93 +264,6 @@ def v2_qdq_backward(grad: torch.Tensor, mask: torch.Tensor, dx: torch.Tensor) ->
 
 
 # ---------------------------------------------------------------------------------------------------
-# layers (matrices [rows, cols] with unit column stride; the callers in v2/nn.py check shapes and devices)
-# ---------------------------------------------------------------------------------------------------
-_ACT = {None: _lib.AQ_ACT_NONE, "relu": _lib.AQ_ACT_RELU, "gelu": _lib.AQ_ACT_GELU, "gelu_tanh": _lib.AQ_ACT_GELU_TANH,
-        "silu": _lib.AQ_ACT_SILU}
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _mat(t: Optional[torch.Tensor]) -> Tuple[Optional[int], int]:
-    """Address and row pitch.  The stride of a dimension of size 1 can be anything; such a row counts as dense."""
-    if t is None:
-        return None, 0
-    rows, cols = t.shape
-    return t.data_ptr(), t.stride(0) if rows > 1 else (cols + 7) // 8 * 8
-
-
-def aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself when the tensor cores can read its rows (see include/aimet_b200.h), else a copy that they can."""
-    if t.dtype is torch.float32:
-        return t
-    ptr, ld = _mat(t)
-    if (ptr % 16 == 0 and ld % 8 == 0) or not t.numel():
-        return t
-    rows, cols = t.shape
-    out = t.new_empty((rows, (cols + 7) // 8 * 8))
-    with _on(t):
-        check(lib.aq_align_rows(ptr, max(ld, cols), out.data_ptr(), out.stride(0), _dt(t), rows, cols, _stream(t)),
-              "aq_align_rows")
-    return out[:, :cols]
-
-
-def linear_forward(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
-                   activation: Optional[str], y: torch.Tensor, z: Optional[torch.Tensor] = None) -> None:
-    with _on(x):
-        check(lib.aq_linear_forward(*_mat(x), *_mat(w), _ptr(bias), *_mat(residual), *_mat(y), *_mat(z), _dt(x),
-                                    x.shape[0], w.shape[0], x.shape[1], _ACT[activation], _stream(x)), "aq_linear_forward")
-
-
-def linear_grad_z(dy: torch.Tensor, z: Optional[torch.Tensor], activation: Optional[str], dz: Optional[torch.Tensor],
-                  dbias: Optional[torch.Tensor]) -> None:
-    m, n = dy.shape
-    dt = _dt(dy)
-    ws, need = None, 0
-    if dbias is not None:
-        need = lib.aq_linear_grad_z_workspace_bytes(dt, m, n)
-        ws = dy.new_empty(need, dtype=torch.uint8)
-    with _on(dy):
-        check(lib.aq_linear_grad_z(*_mat(dy), *_mat(z), *_mat(dz), _ptr(dbias), dt, m, n, _ACT[activation], _ptr(ws), need,
-                                   _stream(dy)), "aq_linear_grad_z")
-
-
-def linear_grad_input(dz: torch.Tensor, w: torch.Tensor, dx: torch.Tensor) -> None:
-    with _on(dz):
-        check(lib.aq_linear_grad_input(*_mat(dz), *_mat(w), *_mat(dx), _dt(dz), dz.shape[0], dz.shape[1], w.shape[1],
-                                       _stream(dz)), "aq_linear_grad_input")
-
-
-def linear_grad_weight(dz: torch.Tensor, x: torch.Tensor, dw: torch.Tensor) -> None:
-    with _on(dz):
-        check(lib.aq_linear_grad_weight(*_mat(dz), *_mat(x), *_mat(dw), _dt(dz), dz.shape[0], dz.shape[1], x.shape[1],
-                                        _stream(dz)), "aq_linear_grad_weight")
-
-
-def layer_norm_forward(x: torch.Tensor, w: Optional[torch.Tensor], b: Optional[torch.Tensor], eps: float,
-                       y: torch.Tensor, mean: Optional[int], rstd: Optional[int]) -> None:
-    """``mean`` / ``rstd``: addresses of one float per row, or None."""
-    with _on(x):
-        check(lib.aq_layer_norm_forward(*_mat(x), _ptr(w), _ptr(b), y.data_ptr(), mean, rstd, _dt(x), x.shape[0], x.shape[1],
-                                        eps, _stream(x)), "aq_layer_norm_forward")
-
-
-def layer_norm_backward(x: torch.Tensor, dy: torch.Tensor, w: Optional[torch.Tensor], mean: int, rstd: int,
-                        dx: Optional[torch.Tensor], dw: Optional[torch.Tensor], db: Optional[torch.Tensor]) -> None:
-    rows, dim = x.shape
-    dt = _dt(x)
-    ws, need = None, 0
-    if dw is not None or db is not None:
-        need = lib.aq_layer_norm_backward_workspace_bytes(dt, rows, dim)
-        ws = x.new_empty(need, dtype=torch.uint8)
-    with _on(x):
-        check(lib.aq_layer_norm_backward(*_mat(x), *_mat(dy), _ptr(w), mean, rstd, _ptr(dx), _ptr(dw), _ptr(db), dt, rows,
-                                         dim, _ptr(ws), need, _stream(x)), "aq_layer_norm_backward")
-
-
-# ---------------------------------------------------------------------------------------------------
 # statistics
 # ---------------------------------------------------------------------------------------------------
 def minmax(x: torch.Tensor, num_ch: int = 1, inner: Optional[int] = None, propagate_nan: bool = False,

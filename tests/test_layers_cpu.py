@@ -66,7 +66,8 @@ def test_python_refuses_cpu_tensors_and_bad_names():
 
 
 def test_rows_views():
-    from aimet_b200.v2.nn import _rows
+    from aimet_b200.v2.nn import _layers
+    _rows = _layers.rows_of
     t = torch.randn(4, 6, 8)
     assert _rows(t, 8).data_ptr() == t.data_ptr() and _rows(t, 8).shape == (24, 8)
     s = torch.randn(4, 6, 16)[..., 4:12]

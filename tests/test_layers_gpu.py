@@ -243,14 +243,21 @@ def test_linear_repeats_bit_for_bit(cuda, dtype):
 
 def test_linear_leaves_its_surroundings_alone(cuda):
     """Results land in freshly allocated memory; what lies around operands and results keeps its bits."""
-    from aimet_b200 import ops
+    from aimet_b200._lib import check, lib
+
+    def forward(x, w, y, z=None):
+        code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[x.dtype]
+        check(lib.aq_linear_forward(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), None, None, 0, y.data_ptr(), y.stride(0),
+                                    None if z is None else z.data_ptr(), 0 if z is None else z.stride(0), code, x.shape[0],
+                                    w.shape[0], x.shape[1], 1, torch.cuda.current_stream().cuda_stream))
+
     for dtype in DTYPES:
         for m, k, n in ((3, 72, 40), (130, 136, 264), (513, 64, 520)):
             g = _gen(37)
             x, w = _randn(g, m, k, dtype=dtype), _randn(g, n, k, dtype=dtype)
             big = torch.full((m + 4, n + 16), 7.0, device=cuda, dtype=dtype)
             zbig = torch.full((m + 4, n + 16), 7.0, device=cuda, dtype=dtype)
-            ops.linear_forward(x, w, None, None, "relu", big[2:2 + m, 8:8 + n], zbig[2:2 + m, 8:8 + n])
+            forward(x, w, big[2:2 + m, 8:8 + n], zbig[2:2 + m, 8:8 + n])
             for t in (big, zbig):
                 edge = t.clone()
                 edge[2:2 + m, 8:8 + n] = 7.0
@@ -258,7 +265,7 @@ def test_linear_leaves_its_surroundings_alone(cuda):
             ref = linear_ref(x, w, None, None, "relu")["y"]
             assert_within(big[2:2 + m, 8:8 + n], ref, "pitched result")
             big = torch.full((m + 4, n + 15), 7.0, device=cuda, dtype=dtype)   # odd pitch, odd start
-            ops.linear_forward(x, w, None, None, "relu", big[2:2 + m, 7:7 + n])
+            forward(x, w, big[2:2 + m, 7:7 + n])
             assert_within(big[2:2 + m, 7:7 + n], ref, "odd result")
             big[2:2 + m, 7:7 + n] = 7.0
             assert bool((big == 7.0).all()), (dtype, m, k, n)
@@ -543,7 +550,7 @@ def test_refusals_on_the_gpu(cuda):
         layer_norm(x, 16, eps=-1.0)
     xr = x.clone().requires_grad_(True)
     (dx,) = torch.autograd.grad(linear(xr, w, None, "silu").sum(), xr, create_graph=True)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(RuntimeError, match="gradients of gradients"):
         dx.sum().backward()
     # the C entry refuses rows the tensor cores cannot read
     h = torch.zeros(12, 24, device=cuda, dtype=torch.float16)

@@ -694,7 +694,7 @@ static inline bool bad_mnk(int64_t m, int64_t n, int64_t k)
 }
 static inline bool huge(int64_t a, int64_t b = 1, int64_t c = 1)
 {
-    const int64_t most = INT32_MAX - 256;   // a last tile still starts and ends inside an int
+    const int64_t most = INT32_MAX - 4096;   // a last tile, and a step beyond the last element, still fit into an int
     return a > most || b > most || c > most;
 }
 

@@ -6,7 +6,7 @@ import torch
 from torch import nn
 import torch.nn.functional as F
 
-from _layers import ACTS, DTYPES, assert_within, act, linear_ref, norm_ref
+from _layers import ACTS, DTYPES, assert_within, act, linear_ref, norm_ref, slope
 
 pytestmark = pytest.mark.gpu
 
@@ -159,6 +159,35 @@ def test_activation_limits(cuda, kind):
     slope = torch.nan_to_num(slope, nan=1.0)   # the formula's 0 * inf at 1e30
     torch.testing.assert_close(y[:, 0].double(), want.detach(), rtol=1e-5, atol=2e-6)
     torch.testing.assert_close(dx[:, 0].double(), slope, rtol=1e-5, atol=2e-6)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=str)
+@pytest.mark.parametrize("kind", ACTS[1:])
+@pytest.mark.parametrize("m,n", [(1, 40), (20, 40), (300, 264), (300, 265)])
+def test_activation_limits_in_16_bits(cuda, kind, dtype, m, n):
+    """The same in the epilogues of the matrix products and in their backward pass, and NaN stays NaN."""
+    from aimet_b200.v2.nn import linear
+    z = torch.tensor([-6e4, -3e3, -200., -50., -14.5, -13.5, -5., -0.5, -1e-3, 0., 1e-3, 0.5, 5., 13.5, 14.5, 50., 200., 6e4],
+                     device=cuda).to(dtype)
+    x = torch.zeros(m, 64, device=cuda, dtype=dtype)
+    w = torch.zeros(n, 64, device=cuda, dtype=dtype)
+    x[:, 3] = 1
+    w[:, 3] = z.repeat(n)[:n]
+    x.requires_grad_(True)
+    b = torch.zeros(n, device=cuda, dtype=dtype, requires_grad=True)
+    y = linear(x, w, b, kind)
+    (db,) = torch.autograd.grad(y, b, torch.cat([torch.ones(1, n, device=cuda), torch.zeros(m - 1, n, device=cuda)]).to(dtype))
+    zz = w[:, 3].double()
+    half = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    # one rounding to the type; the functions themselves are good to 16 steps of 2^-24 of max(1, |z|)
+    want, steep = act(zz, kind), slope(zz, kind)
+    err = (y[0].double() - want).abs()
+    assert bool((err <= half * want.abs() + 16 * 2.0 ** -24 * zz.abs().clamp_min(1)).all())
+    assert bool(((db.double() - steep).abs() <= half * steep.abs() + 32 * 2.0 ** -24).all())
+    bad = x.detach().clone()
+    bad[0, 5] = float("nan")
+    out = linear(bad, w, b.detach(), kind)
+    assert bool(out[0].isnan().all()) and not bool(out[1:].isnan().any())
 
 
 @pytest.mark.parametrize("kind", ACTS)
@@ -522,6 +551,37 @@ def test_two_streams_at_once(cuda):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+
+
+def test_quantized_tensors_count_as_numbers(cuda):
+    """Fake-quantized tensors that carry their encoding: same numbers, plain result, gradients through the quantizer."""
+    from aimet_b200.v2.nn import layer_norm, linear
+    from aimet_b200.v2.quantizer import QuantizeDequantize
+    g = _gen(79)
+    w = _randn(g, 40, 64).requires_grad_(True)
+    q = QuantizeDequantize((40, 1), 8, True).to(cuda)
+    with q.compute_encodings():
+        q(w)
+    wq = q(w)
+    assert type(wq) is not torch.Tensor
+    x = _randn(g, 30, 64)
+    y = linear(x, wq, None, "relu")
+    assert type(y) is torch.Tensor and torch.equal(y, linear(x, wq.detach().as_subclass(torch.Tensor), None, "relu"))
+    (dw,) = torch.autograd.grad(y.sum(), w)
+    assert dw.shape == w.shape and bool(dw.any())
+    assert type(layer_norm(wq, 64)) is torch.Tensor
+
+
+def test_inference_mode_and_backward_accumulation(cuda):
+    from aimet_b200.v2.nn import layer_norm, linear
+    g = _gen(83)
+    x, w = _randn(g, 20, 32), _randn(g, 24, 32).requires_grad_(True)
+    with torch.inference_mode():
+        y = linear(layer_norm(x, 32), w)
+    assert not y.requires_grad
+    for _ in range(2):   # gradients add up in the leaf
+        linear(x, w).sum().backward()
+    torch.testing.assert_close(w.grad, 2 * x.sum(0).expand(24, 32), rtol=1e-5, atol=1e-5)
 
 
 def test_refusals_on_the_gpu(cuda):

@@ -167,14 +167,49 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
             at[1]     = hi;
         }
     tc::cluster_sync();
-    const int e0 = TILE * TILE / kSimtThreads * (int) rank / (int) splits, e1 = TILE * TILE / kSimtThreads * (int) (rank + 1) / (int) splits;
-    for (int s = e0; s < e1; ++s)
+    // every CTA finishes its share of the tile, four neighbouring results per thread at a time
+    constexpr int QUADS = TILE * TILE / 4 / kSimtThreads, AT = 2;
+    const int e0 = QUADS * (int) rank / (int) splits, e1 = QUADS * (int) (rank + 1) / (int) splits;
+#pragma unroll 1
+    for (int q = e0; q < e1; q += AT)
     {
-        const int e = s * kSimtThreads + threadIdx.x;
-        float z     = 0.f;
-        for (uint32_t r = 0; r < splits; ++r)   // always in this order: the same bits on every run
-            z += tc::ld_cluster(tc::map_to(base + e * 4, r));
-        finish(z, i0 + e / TILE, j0 + e % TILE);
+        float4 z[AT];
+#pragma unroll
+        for (int u = 0; u < AT; ++u)
+            z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (uint32_t r = 0; r < splits; r += 4)
+        {
+            float4 w[4][AT];   // on their way together
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int u = 0; u < AT; ++u)
+                    if (r + v < splits && q + u < e1)
+                        w[v][u] = tc::ld_cluster4(tc::map_to(base + ((q + u) * kSimtThreads + threadIdx.x) * 16, r + v));
+#pragma unroll
+            for (int v = 0; v < 4; ++v)   // always in this order: the same bits on every run
+#pragma unroll
+                for (int u = 0; u < AT; ++u)
+                    if (r + v < splits && q + u < e1)
+                    {
+                        z[u].x += w[v][u].x;
+                        z[u].y += w[v][u].y;
+                        z[u].z += w[v][u].z;
+                        z[u].w += w[v][u].w;
+                    }
+        }
+#pragma unroll
+        for (int u = 0; u < AT; ++u)
+            if (q + u < e1)
+            {
+                const int e = ((q + u) * kSimtThreads + threadIdx.x) * 4;
+                const int64_t i = i0 + e / TILE, j = j0 + e % TILE;
+                finish(z[u].x, i, j);
+                finish(z[u].y, i, j + 1);
+                finish(z[u].z, i, j + 2);
+                finish(z[u].w, i, j + 3);
+            }
     }
     tc::cluster_meet();   // nobody leaves while its partial tile may be read
 }
@@ -198,15 +233,20 @@ int simt_gemm(const GemmArgs& a, int splits, cudaStream_t st)
 template <bool AK, bool BK>
 int simt_dispatch(const GemmArgs& a, cudaStream_t st)
 {
-    // Two CTAs per SM.  128 x 128 tiles need half the shared memory traffic per product; 64 x 64 ones with the depth
-    // split come closer to filling the GPU when there are fewer than that many large ones.
+    // Two CTAs per SM.  A 128 x 128 tile costs 0.6 of what its four 64 x 64 ones do, if these CTAs fill at least half of the
+    // GPU's 296 places, with the depth split where the tiles alone do not: 1024^3 59 us in 64 tiles by four, 89 us in 256
+    // small ones; 512 x 4096 -> 4096 404 and 536 us; 128 x 2048 -> 1000, 8 large or 32 small tiles by eight, 39 and 25 us.
+    const int64_t places = 2 * kNumSMs, slices = (a.depth + kDepth - 1) / kDepth;
+    auto splits_for = [&](int64_t tiles, int64_t room) {
+        const int64_t s = room / tiles < slices / 4 ? room / tiles : slices / 4;
+        return s < 1 ? 1 : s > 8 ? 8 : (int) s;
+    };
     const int64_t large = ((a.rows + 127) / 128) * ((a.cols + 127) / 128);
-    if (large >= 2 * kNumSMs)
-        return simt_gemm<128, AK, BK>(a, 1, st);
-    const int64_t small = ((a.rows + 63) / 64) * ((a.cols + 63) / 64), slices = (a.depth + kDepth - 1) / kDepth;
-    int64_t splits = 4 * kNumSMs / small;
-    splits         = splits < slices / 4 ? splits : slices / 4;
-    return simt_gemm<64, AK, BK>(a, (int) (splits < 1 ? 1 : splits > 8 ? 8 : splits), st);
+    const int splits    = splits_for(large, places);
+    if (a.rows > 64 && a.cols > 64 && large * splits >= places / 2)
+        return simt_gemm<128, AK, BK>(a, splits, st);
+    const int64_t small = ((a.rows + 63) / 64) * ((a.cols + 63) / 64);
+    return simt_gemm<64, AK, BK>(a, splits_for(small, 2 * places), st);
 }
 
 int simt_any(const GemmArgs& a, cudaStream_t st)

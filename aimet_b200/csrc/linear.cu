@@ -16,20 +16,23 @@ namespace
 // copies are asynchronous and element-wise: they need no alignment, turn rows into columns on the way, and cost one
 // instruction per 32 fused multiply-adds.
 //
-// TILE x TILE results per CTA of 256 threads, TILE / 16 squared per thread; the depth can be split over a cluster, whose
-// CTAs then add up their partial tiles in a fixed order through distributed shared memory.
+// TM x TN results per CTA of 256 threads, 8 x 8 (128 x 128) or 4 x 4 per thread; the depth can be split over a cluster,
+// whose CTAs then add up their partial tiles in a fixed order through distributed shared memory.
 // ------------------------------------------------------------------------------------------------
 constexpr int kSimtThreads = 256, kDepth = 16;
 
-template <int TILE>
+template <int TM, int TN>
 struct SimtShape
 {
-    static constexpr int kPitch  = TILE + 4;   // [k][row]; the pad spreads the turned copies over the banks
+    static constexpr int kM = TM == 128 ? 8 : 4, kN = TN == 128 && TM == 128 ? 8 : 4;   // results of a thread
+    static constexpr int kTx = TN / kN, kTy = TM / kM;
+    static_assert(kTx * kTy == kSimtThreads, "the threads cover the tile");
+    static constexpr int kPitchA = TM + 4, kPitchB = TN + 4;   // [k][row]; the pad spreads the turned copies over the banks
     static constexpr int kStages = 4;
-    static constexpr int kOffB   = kDepth * kPitch;              // floats
-    static constexpr int kStage  = kOffB + kDepth * kPitch;
+    static constexpr int kOffB   = kDepth * kPitchA;              // floats
+    static constexpr int kStage  = kOffB + kDepth * kPitchB;
     static constexpr int kSmem   = kStages * kStage * 4;
-    static_assert(TILE * TILE * 4 <= kSmem, "the partial tile takes the place of the operands");
+    static_assert(TM * TN * 4 <= kSmem, "the partial tile takes the place of the operands");
 };
 
 __device__ __forceinline__ void copy_async4(uint32_t dst, const float* src, bool in)
@@ -37,12 +40,11 @@ __device__ __forceinline__ void copy_async4(uint32_t dst, const float* src, bool
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
 
-// Slice of TILE rows x 16 k, element (r, c) to dst + c * kPitch + r; what lies outside the matrix (rows beyond
+// Slice of TILE rows x 16 k, element (r, c) to dst + c * PITCH + r; what lies outside the matrix (rows beyond
 // `rows`, k beyond `depth`) becomes 0, and the address then is the start of the slice.
-template <int TILE, bool KMAJOR>
+template <int TILE, int PITCH, bool KMAJOR>
 __device__ __forceinline__ void simt_load(const float* p, int64_t ld, int rows, int depth, uint32_t dst)
 {
-    constexpr int PITCH = SimtShape<TILE>::kPitch;
     constexpr int STEP = KMAJOR ? kSimtThreads / kDepth : kSimtThreads / TILE;   // rows, or k, from one copy to the next
     const int r = KMAJOR ? threadIdx.x / kDepth : threadIdx.x % TILE, c = KMAJOR ? threadIdx.x % kDepth : threadIdx.x / TILE;
     const float* src = p + (KMAJOR ? r * ld + c : c * ld + r);
@@ -57,44 +59,44 @@ __device__ __forceinline__ void simt_load(const float* p, int64_t ld, int rows, 
     }
 }
 
-template <int TILE, bool AK, bool BK, int ACT>
+template <int TM, int TN, bool AK, bool BK, int ACT>
 __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
 {
-    using S         = SimtShape<TILE>;
-    constexpr int M = TILE / 16;   // results per thread and direction: rows ty 4 + {0..3} (+ 64), columns alike
+    using S = SimtShape<TM, TN>;
+    constexpr int M = S::kM, N = S::kN;   // rows ty 4 + {0..3} (and 64 further), columns alike
     extern __shared__ __align__(16) float simt_smem[];
     pdl_launch_dependents();
     uint32_t splits;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
     const uint32_t rank   = tc::cluster_rank();
     const int64_t tile    = blockIdx.x / splits;
-    const int64_t tiles_j = (a.cols + TILE - 1) / TILE;
-    const int64_t i0 = tile / tiles_j * TILE, j0 = tile % tiles_j * TILE;
+    const int64_t tiles_j = (a.cols + TN - 1) / TN;
+    const int64_t i0 = tile / tiles_j * TM, j0 = tile % tiles_j * TN;
     const int64_t slices = (a.depth + kDepth - 1) / kDepth;
     const int64_t s0 = slices * rank / splits, s1 = slices * (rank + 1) / splits;
     const float* pa = (const float*) a.a;
     const float* pb = (const float*) a.b;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int tx = threadIdx.x % S::kTx, ty = threadIdx.x / S::kTx;
     const uint32_t base = tc::smem_addr(simt_smem);
-    const int rows_left = a.rows - i0 < TILE ? (int) (a.rows - i0) : TILE, cols_left = a.cols - j0 < TILE ? (int) (a.cols - j0) : TILE;
+    const int rows_left = a.rows - i0 < TM ? (int) (a.rows - i0) : TM, cols_left = a.cols - j0 < TN ? (int) (a.cols - j0) : TN;
     auto load = [&](int64_t slice) {
         if (slice < s1)
         {
             const uint32_t dst = base + (uint32_t) ((slice - s0) % S::kStages) * S::kStage * 4;
             const int64_t k0   = slice * kDepth;
             const int left     = a.depth - k0 < kDepth ? (int) (a.depth - k0) : kDepth;
-            simt_load<TILE, AK>(pa + (AK ? i0 * a.lda + k0 : k0 * a.lda + i0), a.lda, rows_left, left, dst);
-            simt_load<TILE, BK>(pb + (BK ? j0 * a.ldb + k0 : k0 * a.ldb + j0), a.ldb, cols_left, left,
+            simt_load<TM, S::kPitchA, AK>(pa + (AK ? i0 * a.lda + k0 : k0 * a.lda + i0), a.lda, rows_left, left, dst);
+            simt_load<TN, S::kPitchB, BK>(pb + (BK ? j0 * a.ldb + k0 : k0 * a.ldb + j0), a.ldb, cols_left, left,
                                                dst + S::kOffB * 4);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     pdl_wait();
-    f32x2_t acc[M][M / 2];
+    f32x2_t acc[M][N / 2];
 #pragma unroll
     for (int u = 0; u < M; ++u)
 #pragma unroll
-        for (int v = 0; v < M / 2; ++v)
+        for (int v = 0; v < N / 2; ++v)
             acc[u][v] = pair(0.f, 0.f);
     for (int s = 0; s < S::kStages - 1; ++s)
         load(s0 + s);
@@ -109,19 +111,19 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
         for (int kk = 0; kk < kDepth; ++kk)
         {
             float av[M];
-            ulonglong2 bv[M / 4];   // the register pairs (b0, b1), (b2, b3)
+            ulonglong2 bv[N / 4];   // the register pairs (b0, b1), (b2, b3)
 #pragma unroll
             for (int h = 0; h < M / 4; ++h)
-            {
-                *reinterpret_cast<float4*>(av + 4 * h) = *reinterpret_cast<const float4*>(sa + kk * S::kPitch + 64 * h);
-                bv[h] = *reinterpret_cast<const ulonglong2*>(sb + kk * S::kPitch + 64 * h);
-            }
+                *reinterpret_cast<float4*>(av + 4 * h) = *reinterpret_cast<const float4*>(sa + kk * S::kPitchA + 64 * h);
+#pragma unroll
+            for (int h = 0; h < N / 4; ++h)
+                bv[h] = *reinterpret_cast<const ulonglong2*>(sb + kk * S::kPitchB + 64 * h);
 #pragma unroll
             for (int u = 0; u < M; ++u)
             {
                 const f32x2_t a2 = pair(av[u], av[u]);
 #pragma unroll
-                for (int v = 0; v < M / 2; ++v)
+                for (int v = 0; v < N / 2; ++v)
                     acc[u][v] = fma2(a2, v % 2 ? bv[v / 2].y : bv[v / 2].x, acc[u][v]);
             }
         }
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
 #pragma unroll
         for (int u = 0; u < M; ++u)
 #pragma unroll
-            for (int v = 0; v < M / 2; ++v)
+            for (int v = 0; v < N / 2; ++v)
             {
                 float lo, hi;
                 unpair(acc[u][v], lo, hi);
@@ -158,17 +160,17 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
 #pragma unroll
     for (int u = 0; u < M; ++u)
 #pragma unroll
-        for (int v = 0; v < M / 2; ++v)
+        for (int v = 0; v < N / 2; ++v)
         {
             float lo, hi;
             unpair(acc[u][v], lo, hi);
-            float* at = simt_smem + (u / 4 * 64 + ty * 4 + u % 4) * TILE + v / 2 * 64 + tx * 4 + v % 2 * 2;
+            float* at = simt_smem + (u / 4 * 64 + ty * 4 + u % 4) * TN + v / 2 * 64 + tx * 4 + v % 2 * 2;
             at[0]     = lo;
             at[1]     = hi;
         }
     tc::cluster_sync();
     // every CTA finishes its share of the tile, four neighbouring results per thread at a time
-    constexpr int QUADS = TILE * TILE / 4 / kSimtThreads, AT = 2;
+    constexpr int QUADS = TM * TN / 4 / kSimtThreads, AT = 2;
     const int e0 = QUADS * (int) rank / (int) splits, e1 = QUADS * (int) (rank + 1) / (int) splits;
 #pragma unroll 1
     for (int q = e0; q < e1; q += AT)
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
             if (q + u < e1)
             {
                 const int e = ((q + u) * kSimtThreads + threadIdx.x) * 4;
-                const int64_t i = i0 + e / TILE, j = j0 + e % TILE;
+                const int64_t i = i0 + e / TN, j = j0 + e % TN;
                 finish(z[u].x, i, j);
                 finish(z[u].y, i, j + 1);
                 finish(z[u].z, i, j + 2);
@@ -214,20 +216,24 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
     tc::cluster_meet();   // nobody leaves while its partial tile may be read
 }
 
-template <int TILE, bool AK, bool BK>
+template <int TM, int TN, bool AK, bool BK>
 int simt_gemm(const GemmArgs& a, int splits, cudaStream_t st)
 {
-    const int64_t grid = ((a.rows + TILE - 1) / TILE) * ((a.cols + TILE - 1) / TILE) * splits;
+    const int64_t grid = ((a.rows + TM - 1) / TM) * ((a.cols + TN - 1) / TN) * splits;
     if (grid > 0x7fffffff)
         return AQ_ERR_TOO_LARGE;
-    return with_activation(a.act, [&](auto act) -> int {
-        auto kernel   = simt_gemm_kernel<TILE, AK, BK, decltype(act)::value>;
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SimtShape<TILE>::kSmem);
+    auto run = [&](auto act) -> int {
+        auto kernel   = simt_gemm_kernel<TM, TN, AK, BK, decltype(act)::value>;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SimtShape<TM, TN>::kSmem);
         if (e == cudaSuccess)
-            e = launch_cluster(kernel, (unsigned) grid, splits, kSimtThreads, SimtShape<TILE>::kSmem, st, a);
+            e = launch_cluster(kernel, (unsigned) grid, splits, kSimtThreads, SimtShape<TM, TN>::kSmem, st, a);
         note_launch();
         return e == cudaSuccess ? AQ_OK : cuda_fail(e);
-    });
+    };
+    if constexpr (AK && BK)
+        return with_activation(a.act, run);
+    else   // the backward products have no epilogue
+        return run(std::integral_constant<int, AQ_ACT_NONE> {});
 }
 
 template <bool AK, bool BK>
@@ -244,9 +250,11 @@ int simt_dispatch(const GemmArgs& a, cudaStream_t st)
     const int64_t large = ((a.rows + 127) / 128) * ((a.cols + 127) / 128);
     const int splits    = splits_for(large, places);
     if (a.rows > 64 && a.cols > 64 && large * splits >= places / 2)
-        return simt_gemm<128, AK, BK>(a, splits, st);
+        return simt_gemm<128, 128, AK, BK>(a, splits, st);
+    if (a.rows <= 32)   // half the products of a 64-row tile would be for rows that do not exist
+        return simt_gemm<32, 128, AK, BK>(a, splits_for((a.cols + 127) / 128, 2 * places), st);
     const int64_t small = ((a.rows + 63) / 64) * ((a.cols + 63) / 64);
-    return simt_gemm<64, AK, BK>(a, splits_for(small, 2 * places), st);
+    return simt_gemm<64, 64, AK, BK>(a, splits_for(small, 2 * places), st);
 }
 
 int simt_any(const GemmArgs& a, cudaStream_t st)

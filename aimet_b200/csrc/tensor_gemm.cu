@@ -33,6 +33,7 @@ struct TcArgs
     int a_kmajor, b_kmajor;
     int tiles_i, tiles_j;
     int vec;             // elements per access that out, z and residual allow: 16, 8, or 0
+    int stages;          // slim_kernel
 };
 
 constexpr int kBlockK   = 64;   // one 128-byte row of the swizzle
@@ -434,11 +435,17 @@ template <int BN>
 struct SlimShape
 {
     static constexpr int kStageBytes = 128 * 128 + BN * 128;
-    static constexpr int kStages     = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;   // two CTAs per SM
-    static constexpr int kBars       = kStages * kStageBytes;
-    static constexpr int kSmem       = 1024 + kBars + 256;
+    // shallow: two CTAs per SM; deep: one, with as much of B on its way as the two would have.  (With 16 or 32 rows a deeper
+    // pipeline only crowds the memory: 8 x 4096 -> 11008 24.2 us with twelve stages, 19.4 with six.)
+    static constexpr int kShallow = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
+    static constexpr int kDeep    = BN >= 64 ? 2 * kShallow : kShallow;
+    static constexpr int smem(int stages)
+    {
+        return 1024 + stages * kStageBytes + 256;
+    }
     static constexpr int kTmemCols   = BN < 32 ? 32 : BN;
-    static_assert(BN * 128 * 4 <= kBars, "the partial results of a CTA take the place of its operand tiles");
+    static_assert(BN * 128 * 4 <= kShallow * kStageBytes, "the partial results of a CTA take the place of its operand tiles");
+    static_assert(smem(kDeep) <= 232448 - 16 && 16 * kDeep + 16 <= 256, "shared memory, barriers");
 };
 
 // Four results of row i from column j.  With p.vec every row starts on a 16-byte boundary and the number of columns is a
@@ -500,8 +507,9 @@ __global__ void __launch_bounds__(192, 2)
     __shared__ int stuck_smem;
     volatile int* stuck = &stuck_smem;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-    const uint32_t bars = base + S::kBars;
-    const uint32_t full = bars, empty = full + 8 * S::kStages, tfull = empty + 8 * S::kStages, tmem_at = tfull + 8;
+    const int stages    = p.stages;
+    const uint32_t bars = base + stages * S::kStageBytes;
+    const uint32_t full = bars, empty = full + 8 * stages, tfull = empty + 8 * stages, tmem_at = tfull + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t splits;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
@@ -511,7 +519,7 @@ __global__ void __launch_bounds__(192, 2)
     if (threadIdx.x == 0)
     {
         stuck_smem = 0;
-        for (int s = 0; s < S::kStages; ++s)
+        for (int s = 0; s < stages; ++s)
         {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
@@ -565,7 +573,7 @@ __global__ void __launch_bounds__(192, 2)
                 }
             }
             __syncwarp();
-            if (++s == S::kStages)
+            if (++s == stages)
             {
                 s = 0;
                 phase ^= 1u;
@@ -593,7 +601,7 @@ __global__ void __launch_bounds__(192, 2)
                     mma_commit(tfull);
             }
             __syncwarp();
-            if (++s == S::kStages)
+            if (++s == stages)
             {
                 s = 0;
                 phase ^= 1u;
@@ -817,6 +825,7 @@ int run_pair(const GemmArgs& a, cudaStream_t st)
 template <typename T, int BN>
 int run_slim(const GemmArgs& a, int splits, cudaStream_t st)
 {
+    using S = SlimShape<BN>;
     CUtensorMap ma, mb;
     int rc = operand_map(&ma, a.a, a.lda, a.a_kmajor, a.rows, a.depth, BN, a.dtype);
     if (rc == AQ_OK)
@@ -828,8 +837,10 @@ int run_slim(const GemmArgs& a, int splits, cudaStream_t st)
     p.tiles_j = (int) ((a.cols + 127) / 128);
     p.vec     = wide_access(a);
     // the columns' operand is the instruction's A
-    p.idesc = instruction_desc(a.dtype == AQ_BF16, a.b_kmajor, a.a_kmajor, 128, BN);
-    return launch(slim_kernel<T, BN>, (int64_t) p.tiles_i * p.tiles_j * splits, splits, 192, SlimShape<BN>::kSmem, st, ma, mb, p);
+    p.idesc            = instruction_desc(a.dtype == AQ_BF16, a.b_kmajor, a.a_kmajor, 128, BN);
+    const int64_t ctas = (int64_t) p.tiles_i * p.tiles_j * splits;
+    p.stages           = ctas <= kNumSMs ? S::kDeep : S::kShallow;
+    return launch(slim_kernel<T, BN>, ctas, splits, 192, S::smem(p.stages), st, ma, mb, p);
 }
 
 // Clusters of `splits` CTAs of slim_kernel that the current device holds at once (a cluster lives inside one GPC, so this
@@ -844,11 +855,11 @@ int resident_clusters(int splits)
     int n = known[dev][splits].load(std::memory_order_relaxed);
     if (n == 0)
     {
-        cudaFuncSetAttribute(slim_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SlimShape<BN>::kSmem);
+        cudaFuncSetAttribute(slim_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SlimShape<BN>::smem(SlimShape<BN>::kShallow));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim            = dim3(splits);
         cfg.blockDim           = dim3(192);
-        cfg.dynamicSmemBytes   = SlimShape<BN>::kSmem;
+        cfg.dynamicSmemBytes   = SlimShape<BN>::smem(SlimShape<BN>::kShallow);
         cudaLaunchAttribute attr[1];
         attr[0].id               = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = splits;

@@ -16,17 +16,16 @@ namespace
 // copies are asynchronous and element-wise: they need no alignment, turn rows into columns on the way, and cost one
 // instruction per 32 fused multiply-adds.
 //
-// TM x TN results per CTA of 256 threads, 8 x 8 (128 x 128) or 4 x 4 per thread; the depth can be split over a cluster,
+// TM x TN results per CTA, 8 x 16 (128 x 128) or 4 x 4 per thread; the depth can be split over a cluster,
 // whose CTAs then add up their partial tiles in a fixed order through distributed shared memory.
 // ------------------------------------------------------------------------------------------------
-constexpr int kSimtThreads = 256, kDepth = 16;
+constexpr int kDepth = 16;
 
 template <int TM, int TN>
 struct SimtShape
 {
-    static constexpr int kM = TM == 128 ? 8 : 4, kN = TN == 128 && TM == 128 ? 8 : 4;   // results of a thread
-    static constexpr int kTx = TN / kN, kTy = TM / kM;
-    static_assert(kTx * kTy == kSimtThreads, "the threads cover the tile");
+    static constexpr int kM = TM == 128 ? 8 : 4, kN = TM == 128 ? 16 : 4;   // results of a thread
+    static constexpr int kTx = TN / kN, kTy = TM / kM, kThreads = kTx * kTy;
     static constexpr int kPitchA = TM + 4, kPitchB = TN + 4;   // [k][row]; the pad spreads the turned copies over the banks
     static constexpr int kStages = 4;
     static constexpr int kOffB   = kDepth * kPitchA;              // floats
@@ -42,15 +41,15 @@ __device__ __forceinline__ void copy_async4(uint32_t dst, const float* src, bool
 
 // Slice of TILE rows x 16 k, element (r, c) to dst + c * PITCH + r; what lies outside the matrix (rows beyond
 // `rows`, k beyond `depth`) becomes 0, and the address then is the start of the slice.
-template <int TILE, int PITCH, bool KMAJOR>
+template <int TILE, int PITCH, int THREADS, bool KMAJOR>
 __device__ __forceinline__ void simt_load(const float* p, int64_t ld, int rows, int depth, uint32_t dst)
 {
-    constexpr int STEP = KMAJOR ? kSimtThreads / kDepth : kSimtThreads / TILE;   // rows, or k, from one copy to the next
+    constexpr int STEP = KMAJOR ? THREADS / kDepth : THREADS / TILE;   // rows, or k, from one copy to the next
     const int r = KMAJOR ? threadIdx.x / kDepth : threadIdx.x % TILE, c = KMAJOR ? threadIdx.x % kDepth : threadIdx.x / TILE;
     const float* src = p + (KMAJOR ? r * ld + c : c * ld + r);
     uint32_t at      = dst + (c * PITCH + r) * 4;
 #pragma unroll
-    for (int s = 0; s < TILE * kDepth / kSimtThreads; ++s)
+    for (int s = 0; s < TILE * kDepth / THREADS; ++s)
     {
         const bool in = KMAJOR ? r + s * STEP < rows && c < depth : r < rows && c + s * STEP < depth;
         copy_async4(at, in ? src : p, in);
@@ -60,10 +59,10 @@ __device__ __forceinline__ void simt_load(const float* p, int64_t ld, int rows, 
 }
 
 template <int TM, int TN, bool AK, bool BK, int ACT>
-__global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
+__global__ void __launch_bounds__(SimtShape<TM, TN>::kThreads, 2) simt_gemm_kernel(GemmArgs a)
 {
     using S = SimtShape<TM, TN>;
-    constexpr int M = S::kM, N = S::kN;   // rows ty 4 + {0..3} (and 64 further), columns alike
+    constexpr int M = S::kM, N = S::kN;   // rows ty 4 + {0..3} (and 4 kTy further), columns alike
     extern __shared__ __align__(16) float simt_smem[];
     pdl_launch_dependents();
     uint32_t splits;
@@ -85,8 +84,8 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
             const uint32_t dst = base + (uint32_t) ((slice - s0) % S::kStages) * S::kStage * 4;
             const int64_t k0   = slice * kDepth;
             const int left     = a.depth - k0 < kDepth ? (int) (a.depth - k0) : kDepth;
-            simt_load<TM, S::kPitchA, AK>(pa + (AK ? i0 * a.lda + k0 : k0 * a.lda + i0), a.lda, rows_left, left, dst);
-            simt_load<TN, S::kPitchB, BK>(pb + (BK ? j0 * a.ldb + k0 : k0 * a.ldb + j0), a.ldb, cols_left, left,
+            simt_load<TM, S::kPitchA, S::kThreads, AK>(pa + (AK ? i0 * a.lda + k0 : k0 * a.lda + i0), a.lda, rows_left, left, dst);
+            simt_load<TN, S::kPitchB, S::kThreads, BK>(pb + (BK ? j0 * a.ldb + k0 : k0 * a.ldb + j0), a.ldb, cols_left, left,
                                                dst + S::kOffB * 4);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -114,10 +113,10 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
             ulonglong2 bv[N / 4];   // the register pairs (b0, b1), (b2, b3)
 #pragma unroll
             for (int h = 0; h < M / 4; ++h)
-                *reinterpret_cast<float4*>(av + 4 * h) = *reinterpret_cast<const float4*>(sa + kk * S::kPitchA + 64 * h);
+                *reinterpret_cast<float4*>(av + 4 * h) = *reinterpret_cast<const float4*>(sa + kk * S::kPitchA + 4 * S::kTy * h);
 #pragma unroll
             for (int h = 0; h < N / 4; ++h)
-                bv[h] = *reinterpret_cast<const ulonglong2*>(sb + kk * S::kPitchB + 64 * h);
+                bv[h] = *reinterpret_cast<const ulonglong2*>(sb + kk * S::kPitchB + 4 * S::kTx * h);
 #pragma unroll
             for (int u = 0; u < M; ++u)
             {
@@ -150,7 +149,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
             {
                 float lo, hi;
                 unpair(acc[u][v], lo, hi);
-                const int64_t i = i0 + u / 4 * 64 + ty * 4 + u % 4, j = j0 + v / 2 * 64 + tx * 4 + v % 2 * 2;
+                const int64_t i = i0 + u / 4 * 4 * S::kTy + ty * 4 + u % 4, j = j0 + v / 2 * 4 * S::kTx + tx * 4 + v % 2 * 2;
                 finish(lo, i, j);
                 finish(hi, i, j + 1);
             }
@@ -164,13 +163,13 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
         {
             float lo, hi;
             unpair(acc[u][v], lo, hi);
-            float* at = simt_smem + (u / 4 * 64 + ty * 4 + u % 4) * TN + v / 2 * 64 + tx * 4 + v % 2 * 2;
+            float* at = simt_smem + (u / 4 * 4 * S::kTy + ty * 4 + u % 4) * TN + v / 2 * 4 * S::kTx + tx * 4 + v % 2 * 2;
             at[0]     = lo;
             at[1]     = hi;
         }
     tc::cluster_sync();
     // every CTA finishes its share of the tile, four neighbouring results per thread at a time
-    constexpr int QUADS = TM * TN / 4 / kSimtThreads, AT = 2;
+    constexpr int THREADS = S::kThreads, QUADS = TM * TN / 4 / THREADS, AT = 2;
     const int e0 = QUADS * (int) rank / (int) splits, e1 = QUADS * (int) (rank + 1) / (int) splits;
 #pragma unroll 1
     for (int q = e0; q < e1; q += AT)
@@ -188,7 +187,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
 #pragma unroll
                 for (int u = 0; u < AT; ++u)
                     if (r + v < splits && q + u < e1)
-                        w[v][u] = tc::ld_cluster4(tc::map_to(base + ((q + u) * kSimtThreads + threadIdx.x) * 16, r + v));
+                        w[v][u] = tc::ld_cluster4(tc::map_to(base + ((q + u) * THREADS + threadIdx.x) * 16, r + v));
 #pragma unroll
             for (int v = 0; v < 4; ++v)   // always in this order: the same bits on every run
 #pragma unroll
@@ -205,7 +204,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) simt_gemm_kernel(GemmArgs a)
         for (int u = 0; u < AT; ++u)
             if (q + u < e1)
             {
-                const int e = ((q + u) * kSimtThreads + threadIdx.x) * 4;
+                const int e = ((q + u) * THREADS + threadIdx.x) * 4;
                 const int64_t i = i0 + e / TN, j = j0 + e % TN;
                 finish(z[u].x, i, j);
                 finish(z[u].y, i, j + 1);
@@ -226,7 +225,7 @@ int simt_gemm(const GemmArgs& a, int splits, cudaStream_t st)
         auto kernel   = simt_gemm_kernel<TM, TN, AK, BK, decltype(act)::value>;
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SimtShape<TM, TN>::kSmem);
         if (e == cudaSuccess)
-            e = launch_cluster(kernel, (unsigned) grid, splits, kSimtThreads, SimtShape<TM, TN>::kSmem, st, a);
+            e = launch_cluster(kernel, (unsigned) grid, splits, SimtShape<TM, TN>::kThreads, SimtShape<TM, TN>::kSmem, st, a);
         note_launch();
         return e == cudaSuccess ? AQ_OK : cuda_fail(e);
     };

@@ -239,8 +239,8 @@ template <bool AK, bool BK>
 int simt_dispatch(const GemmArgs& a, cudaStream_t st)
 {
     // Two CTAs per SM.  A 128 x 128 tile costs 0.6 of what its four 64 x 64 ones do, if these CTAs fill at least half of the
-    // GPU's 296 places, with the depth split where the tiles alone do not: 1024^3 59 us in 64 tiles by four, 89 us in 256
-    // small ones; 512 x 4096 -> 4096 404 and 536 us; 128 x 2048 -> 1000, 8 large or 32 small tiles by eight, 39 and 25 us.
+    // GPU's 296 places, with the depth split where the tiles alone do not: 1024^3 56 us in 64 tiles by four, 86 us in 256
+    // small ones; 512 x 4096 -> 4096 390 and 648 us; 128 x 2048 -> 1000, 8 large or 32 small tiles by eight, 37 and 26 us.
     const int64_t places = 2 * kNumSMs, slices = (a.depth + kDepth - 1) / kDepth;
     auto splits_for = [&](int64_t tiles, int64_t room) {
         const int64_t s = room / tiles < slices / 4 ? room / tiles : slices / 4;

@@ -9,12 +9,15 @@
 //
 // Which kernel takes a call:
 //   norm_fwd_kernel        forward, a row in the registers of 4 to 512 threads
+//   norm_fwd_any_kernel    the same in 16-byte packets for many long rows off 16-byte boundaries
 //   norm_bwd_ring_kernel   backward: rows arrive in shared memory by bulk copies, several ahead; the sums for dw and db
 //                          stay in registers
-//   norm_bwd_kernel        backward of short rows and of rows without 16-byte boundaries: the next row is fetched into
+//   norm_bwd_kernel        backward of short rows, and of few rows off 16-byte boundaries: the next row is fetched into
 //                          registers instead
 //   *_loop_kernel, norm_param_kernel   rows too long for the registers of 512 threads
 // (A forward ring was slower than enough rows in registers: 16384 x 4096 bf16 53 us against 46.)
+#include <cfloat>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "tensor_core.cuh"
@@ -140,6 +143,100 @@ __device__ __forceinline__ void store_row(const Pack<T, VEC> (&p)[PACKS], T* row
     }
 }
 
+// ---- rows that do not start or end on 16-byte boundaries -----------------------------------------------------------
+// Packets are laid on the 16-byte boundaries of the row that is written.  What is left before the first and behind the last
+// of them, fewer than VEC elements each, goes to the first 2 VEC threads, one element each: with packets that were in part
+// outside the row, the warps that held them set the pace (16384 x 4097 bf16 forward 138 us, backward 146 us).  An input
+// with other boundaries is read as the two aligned pieces that hold a packet.  Now 78 and 105 us (float32 93 and 140);
+// element by element 196 and 369 us (175 and 292).
+struct Cut
+{
+    int head, end;   // the packets hold elements head to end - 1
+    int mine;        // this thread's single element, -1 without one
+
+    template <typename T>
+    static __device__ __forceinline__ Cut of(const T* row, int t, int dim)
+    {
+        constexpr int VEC = 16 / (int) sizeof(T);
+        Cut c;
+        c.head = (VEC - (int) ((uintptr_t) row % 16 / sizeof(T))) % VEC;
+        c.end  = c.head + (dim - c.head) / VEC * VEC;
+        c.mine = t < c.head ? t : t >= VEC && t - VEC < dim - c.end ? c.end + t - VEC : -1;
+        return c;
+    }
+};
+// Elements of T between the last 16-byte boundary and p.
+template <typename T>
+__device__ __forceinline__ int elements_in(const T* p)
+{
+    return (int) ((uintptr_t) p % 16 / sizeof(T));
+}
+// 16 of the 32 bytes (lo, hi), from byte `from` (0 to 15, even) on
+__device__ __forceinline__ uint4 piece(uint4 lo, uint4 hi, uint32_t from)
+{
+    uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int j = 0; j < 6; ++j)
+        u[j] = from & 8 ? u[j + 2] : u[j];
+#pragma unroll
+    for (int j = 0; j < 5; ++j)
+        u[j] = from & 4 ? u[j + 1] : u[j];
+    const uint32_t bits = (from & 2) * 8;
+    return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits), __funnelshift_r(u[2], u[3], bits),
+                      __funnelshift_r(u[3], u[4], bits));
+}
+// The packets at at[k] < end of p, by the element.
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void load_elements(Pack<T, VEC> (&r)[N], const T* p, const int (&at)[N], int end, float fill)
+{
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+    {
+        r[k] = splat<T, VEC>(fill);
+        if (p && at[k] < end)
+#pragma unroll
+            for (int c = 0; c < VEC; ++c)
+                r[k].v[c] = p[at[k] + c];
+    }
+}
+// The packets of a row, and zeros.  Between two other rows that lie at least 2 VEC elements from it whole pieces are read:
+// what they hold besides the packets lies between elements of x.
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void load_row_any(uint4 (&r)[N], const T* row, const int (&at)[N], int end, bool between)
+{
+    if (!between)
+    {
+        Pack<T, VEC> p[N];
+        load_elements(p, row, at, end, 0.f);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            memcpy(&r[k], &p[k], 16);
+        return;
+    }
+    const int off = elements_in(row + at[0]);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+    {
+        r[k] = make_uint4(0, 0, 0, 0);
+        if (at[k] < end)
+            r[k] = *reinterpret_cast<const uint4*>(row + at[k] - off);
+    }
+    if (off)
+    {
+        uint4 hi[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+        {
+            hi[k] = make_uint4(0, 0, 0, 0);
+            if (at[k] < end)
+                hi[k] = *reinterpret_cast<const uint4*>(row + at[k] - off + VEC);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            r[k] = piece(r[k], hi[k], off * sizeof(T));
+    }
+}
+
 // Statistics and result of a row whose packets are in v.  w and b come out of L1.  The arithmetic runs two float32 lanes per instruction.
 template <typename T, int VEC, int TPR, int PACKS>
 __device__ __forceinline__ void norm_row(const LayerNormArgs& a, const Pack<T, VEC> (&v)[PACKS], int64_t row, int t,
@@ -219,6 +316,99 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(LayerNo
     norm_row<T, VEC, TPR>(a, v, row, t, red, live);
 }
 
+// The same for rows off 16-byte boundaries.  A group of threads keeps its columns from row to row (the rows it takes are a
+// multiple of 16 bytes apart), so it reads and shifts its part of w and b once; the next row is on its way while one is
+// reduced.  4000 x 5001 bf16 34 us in 320 threads with two packets each, 40 us in 192 with four.
+template <int TPR, int PACKS>
+struct AnyShape
+{
+    static constexpr int kThreads = TPR < 128 ? 128 : TPR;
+    static constexpr int kRows    = TPR < 128 ? 128 / TPR : 1;
+    static constexpr int kCtas    = ctas_for(16 * PACKS + 48, kThreads);
+};
+
+template <typename T, int TPR, int PACKS>
+__global__ void __launch_bounds__(AnyShape<TPR, PACKS>::kThreads, AnyShape<TPR, PACKS>::kCtas) norm_fwd_any_kernel(LayerNormArgs a)
+{
+    constexpr int VEC = 16 / (int) sizeof(T), ROWS = AnyShape<TPR, PACKS>::kRows;
+    __shared__ float4 red[2][8];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t          = threadIdx.x % TPR, dim = (int) a.dim;
+    const int64_t stride = (int64_t) gridDim.x * ROWS;
+    int64_t row          = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR;
+    const Cut cut        = Cut::of((const T*) a.y + row * a.dim, t, dim);
+    int at[PACKS];
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k)
+        at[k] = cut.head + (k * TPR + t) * VEC;
+    Pack<T, VEC> w[PACKS], b[PACKS];
+    load_elements(w, (const T*) a.w, at, cut.end, 1.f);
+    load_elements(b, (const T*) a.b, at, cut.end, 0.f);
+    const bool one_more = cut.mine >= 0;
+    const float w1 = one_more && a.w ? to_f32(((const T*) a.w)[cut.mine]) : 1.f;
+    const float b1 = one_more && a.b ? to_f32(((const T*) a.b)[cut.mine]) : 0.f;
+    uint4 next[PACKS];
+    T next1    = from_f32<T>(0.f);
+    auto fetch = [&](int64_t r) {
+        const T* x = (const T*) a.x + r * a.ldx;
+        load_row_any<T, VEC>(next, x, at, cut.end, r > 0 && r + 1 < a.rows);
+        if (one_more)
+            next1 = x[cut.mine];
+    };
+    if (row < a.rows)
+        fetch(row);
+    for (; row < a.rows; row += stride)
+    {
+        Pack<T, VEC> v[PACKS];
+        memcpy(v, next, sizeof(v));
+        const float x1 = to_f32(next1);
+        if (row + stride < a.rows)
+            fetch(row + stride);
+        f32x2_t s2 = pair(x1, 0.f);
+#pragma unroll
+        for (int q = 0; q < PACKS * VEC / 2; ++q)
+            s2 = add2(s2, lanes(v, q));
+        const float mu   = row_sum2<TPR>(lane_sum(s2), 0.f, red[0]).x / (float) a.dim;
+        const f32x2_t m2 = pair(mu, mu);
+        const float d1   = one_more ? x1 - mu : 0.f;
+        s2               = pair(d1 * d1, 0.f);
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k)
+            if (at[k] < cut.end)   // the others hold zeros, not the mean
+            {
+                const Pack<T, VEC> one[1] = {v[k]};
+#pragma unroll
+                for (int q = 0; q < VEC / 2; ++q)
+                {
+                    const f32x2_t d = sub2(lanes(one, q), m2);
+                    s2              = fma2(d, d, s2);
+                }
+            }
+        const float rstd = 1.f / sqrtf(row_sum2<TPR>(lane_sum(s2), 0.f, red[1]).x / (float) a.dim + a.eps);
+        const f32x2_t r2 = pair(rstd, rstd);
+        T* y             = (T*) a.y + row * a.dim;
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k)
+            if (at[k] < cut.end)
+            {
+                const Pack<T, VEC> one[1] = {v[k]}, wk[1] = {w[k]}, bk[1] = {b[k]};
+                Pack<T, VEC> o[1];
+#pragma unroll
+                for (int q = 0; q < VEC / 2; ++q)
+                    set_lanes(o, q, fma2(mul2(sub2(lanes(one, q), m2), r2), lanes(wk, q), lanes(bk, q)));
+                store_pack<T, VEC>(y + at[k], o[0]);
+            }
+        if (one_more)
+            y[cut.mine] = from_f32<T>(fmaf(d1 * rstd, w1, b1));
+        if (t == 0 && a.mean)
+        {
+            a.mean[row] = mu;
+            a.rstd[row] = rstd;
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------
 // Backward with a ring of rows in shared memory.  One thread of a row's group (a warp, or the CTA) keeps
 // `stages` rows on their way with bulk copies, so that the memory system sees 100 to 200 KB in flight per SM however
@@ -235,32 +425,82 @@ struct RingShape
     static_assert(kGroups == 1 || TPR == 32, "a row belongs to a warp or to the CTA");
 };
 
-// dynamic shared memory: [group][stage][MATRICES][dim] of T, then the barriers [group][stage]
-template <typename T, int MATRICES>
+// Bytes of a row of the ring: in a ring of any rows 16 in front and 16 behind (the two pieces of a packet may begin before
+// the row and end after it), and the row from a 16-byte boundary to another.
+__host__ __device__ constexpr int64_t ring_row_bytes(int64_t bytes, bool any)
+{
+    return any ? (bytes + 15) / 16 * 16 + 80 : bytes;
+}
+
+// dynamic shared memory: [group][stage][x, dy][ring_row_bytes], then the barriers [group][stage]
+template <typename T, bool ANY>
 struct Ring
 {
-    uint32_t data, bars, row_bytes;
+    uint32_t data, bars, row_bytes, pitch;
     int stages, stage = 0;
     uint32_t phase    = 0;
     volatile int* stuck;
 
     __device__ __forceinline__ Ring(uint32_t base, int groups, int group, int stages_, int64_t dim, volatile int* stuck_)
-        : row_bytes((uint32_t) dim * sizeof(T)), stages(stages_), stuck(stuck_)
+        : row_bytes((uint32_t) dim * sizeof(T)), pitch((uint32_t) ring_row_bytes(dim * sizeof(T), ANY)), stages(stages_),
+          stuck(stuck_)
     {
-        data = base + group * stages * MATRICES * row_bytes;
-        bars = base + groups * stages * MATRICES * row_bytes + group * stages * 8;
+        data = base + group * stages * 2 * pitch;
+        bars = base + groups * stages * 2 * pitch + group * stages * 8;
     }
+    // where the row, or the 16-byte boundary before it, lies
     __device__ __forceinline__ uint32_t at(int s, int matrix) const
     {
-        return data + (s * MATRICES + matrix) * row_bytes;
+        return data + (s * 2 + matrix) * pitch + (ANY ? 16 : 0);
     }
-    __device__ __forceinline__ void request(int s, const T* p0, const T* p1 = nullptr)
+    __device__ __forceinline__ void request(int s, const T* p0, const T* p1)
     {
         const uint32_t bar = bars + 8 * s;
-        tc::mbar_expect(bar, MATRICES * row_bytes);
+        tc::mbar_expect(bar, 2 * row_bytes);
         tc::bulk_load(at(s, 0), p0, row_bytes, bar);
-        if (MATRICES == 2)
-            tc::bulk_load(at(s, 1), p1, row_bytes, bar);
+        tc::bulk_load(at(s, 1), p1, row_bytes, bar);
+    }
+    // Rows off the boundaries.  Between two other rows the copy takes whole pieces, with some of its neighbours' elements
+    // (or what lies between them); of the first and the last row it takes the whole pieces inside, and this thread the rest.
+    __device__ __forceinline__ void request_any(int s, const T* p0, const T* p1, bool between)
+    {
+        const T* p[2] = {p0, p1};
+        uintptr_t from[2];
+        uint32_t bytes[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+            const uintptr_t begin = (uintptr_t) p[i], end = begin + row_bytes;
+            from[i]               = between ? begin / 16 * 16 : (begin + 15) / 16 * 16;
+            const uintptr_t to    = between ? (end + 15) / 16 * 16 : end / 16 * 16;
+            bytes[i]              = (uint32_t) (to - from[i]);
+            if (!between)
+            {
+                const uint32_t row = at(s, i) + (uint32_t) (begin % 16);
+                for (uintptr_t e = begin; e < from[i]; e += sizeof(T))
+                    put(row + (uint32_t) (e - begin), *reinterpret_cast<const T*>(e));
+                for (uintptr_t e = to; e < end; e += sizeof(T))
+                    put(row + (uint32_t) (e - begin), *reinterpret_cast<const T*>(e));
+            }
+        }
+        if (!between)   // a later copy may write there
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        const uint32_t bar = bars + 8 * s;
+        tc::mbar_expect(bar, bytes[0] + bytes[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            tc::bulk_load(at(s, i) + (uint32_t) (from[i] - (uintptr_t) p[i] / 16 * 16), (const void*) from[i], bytes[i], bar);
+    }
+    static __device__ __forceinline__ void put(uint32_t at, T v)
+    {
+        if constexpr (sizeof(T) == 2)
+        {
+            uint16_t u;
+            memcpy(&u, &v, 2);
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(u) : "memory");
+        }
+        else
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
     }
     __device__ __forceinline__ bool wait()
     {
@@ -276,20 +516,40 @@ struct Ring
     }
 };
 
-template <typename T, int VEC, int TPR, int PACKS>
-__device__ __forceinline__ void read_row(Pack<T, VEC> (&p)[PACKS], uint32_t row, int t, int64_t dim)
+__device__ __forceinline__ uint4 shared16(uint32_t at)
 {
-#pragma unroll
-    for (int k = 0; k < PACKS; ++k)
+    uint4 u;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
+    return u;
+}
+// Elements i and on of the row whose first one lies at `row` in shared memory
+template <typename T, int VEC, bool ANY>
+__device__ __forceinline__ Pack<T, VEC> read_packet(uint32_t row, int i)
+{
+    const uint32_t at = row + i * (uint32_t) sizeof(T), off = ANY ? at % 16 : 0;
+    uint4 u           = shared16(at - off);
+    if (off)
+        u = piece(u, shared16(at - off + 16), off);
+    Pack<T, VEC> p;
+    memcpy(&p, &u, 16);
+    return p;
+}
+template <typename T>
+__device__ __forceinline__ float read_element(uint32_t row, int i)
+{
+    if constexpr (sizeof(T) == 4)
     {
-        const int i = (k * TPR + t) * VEC;
-        uint4 u     = make_uint4(0, 0, 0, 0);
-        if (i < dim)
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                         : "r"(row + i * (uint32_t) sizeof(T))
-                         : "memory");
-        memcpy(&p[k], &u, 16);
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(row + i * 4) : "memory");
+        return v;
+    }
+    else
+    {
+        uint16_t u;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(row + i * 2) : "memory");
+        T v;
+        memcpy(&v, &u, 2);
+        return to_f32(v);
     }
 }
 
@@ -306,7 +566,8 @@ struct BwdColumns
     static constexpr int kRegs = (KEEP ? 4 : 2) * N + 48;
 };
 
-template <typename T, int TPR, int PACKS>
+// ANY: rows off 16-byte boundaries.  The rows of a group are a multiple of 16 bytes apart, so that it keeps its columns.
+template <typename T, int TPR, int PACKS, bool ANY>
 __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<T, PACKS>::kRegs, RingShape<TPR>::kThreads))
     norm_bwd_ring_kernel(LayerNormGradArgs a, int stages)
 {
@@ -317,7 +578,7 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
     __shared__ float4 red[2][8];
     __shared__ int stuck_smem;
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    Ring<T, 2> ring(tc::smem_addr(ring_smem), GROUPS, group, stages, a.dim, &stuck_smem);
+    Ring<T, ANY> ring(tc::smem_addr(ring_smem), GROUPS, group, stages, a.dim, &stuck_smem);
     pdl_launch_dependents();
     if (threadIdx.x == 0)
         stuck_smem = 0;
@@ -329,8 +590,21 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
     const int64_t stride = (int64_t) gridDim.x * GROUPS;
     int64_t row          = (int64_t) blockIdx.x * GROUPS + group;
     auto request         = [&](int s, int64_t r) {
-        ring.request(s, (const T*) a.x + r * a.ldx, (const T*) a.dy + r * a.lddy);
+        const T *x = (const T*) a.x + r * a.ldx, *dy = (const T*) a.dy + r * a.lddy;
+        if constexpr (ANY)
+            ring.request_any(s, x, dy, r > 0 && r + 1 < a.rows);
+        else
+            ring.request(s, x, dy);
     };
+    const int dim  = (int) a.dim;
+    Cut cut        = {0, dim, -1};
+    uint32_t off_x = 0, off_g = 0;   // bytes of the rows behind a boundary
+    if constexpr (ANY)
+    {
+        off_x = (uint32_t) elements_in((const T*) a.x + row * a.ldx) * sizeof(T);
+        off_g = (uint32_t) elements_in((const T*) a.dy + row * a.lddy) * sizeof(T);
+        cut   = Cut::of(a.dx ? (const T*) a.dx + row * a.dim : (const T*) a.x + row * a.ldx, t, dim);
+    }
     // a stage is requested again behind the barrier of the row that it held, or, if dx is formed from it after that barrier,
     // behind the next row's
     constexpr bool LATE = !KEEP && GROUPS == 1;
@@ -344,7 +618,19 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
     for (int q = 0; q < Q; ++q)
         dw[q] = db[q] = zero;
     Pack<T, VEC> w[PACKS];
-    load_row<T, VEC, TPR>(w, (const T*) a.w, t, a.dim, 1.f);
+    if constexpr (ANY)
+    {
+        int at[PACKS];
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k)
+            at[k] = cut.head + (k * TPR + t) * VEC;
+        load_elements(w, (const T*) a.w, at, cut.end, 1.f);
+    }
+    else
+        load_row<T, VEC, TPR>(w, (const T*) a.w, t, a.dim, 1.f);
+    const bool one_more = ANY && cut.mine >= 0;
+    const float w1      = one_more && a.w ? to_f32(((const T*) a.w)[cut.mine]) : 1.f;
+    float dw1 = 0.f, db1 = 0.f;
     float mu = 0.f, rstd = 0.f;
     if (row < a.rows)
     {
@@ -353,7 +639,7 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
     }
     for (int slot = 0; row < a.rows; row += stride, slot ^= 1)
     {
-        const float r    = rstd;
+        const float r = rstd, mean = mu;
         const f32x2_t m2 = pair(mu, mu), r2 = pair(r, r);
         if (row + stride < a.rows)
         {
@@ -361,14 +647,25 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
             rstd = a.rstd[row + stride];
         }
         const bool ok = ring.wait();
-        const uint32_t at_x = ring.at(ring.stage, 0), at_g = ring.at(ring.stage, 1);
-        f32x2_t sg = zero, sgh = zero, kept_h[KEEP ? Q : 1], kept_g[KEEP ? Q : 1];
+        const uint32_t at_x = ring.at(ring.stage, 0) + off_x, at_g = ring.at(ring.stage, 1) + off_g;
+        float h1 = 0.f, g1 = 0.f;
+        if (one_more)
+        {
+            const float dy = read_element<T>(at_g, cut.mine);
+            h1             = (read_element<T>(at_x, cut.mine) - mean) * r;
+            g1             = dy * w1;
+            dw1            = fmaf(dy, h1, dw1);
+            db1 += dy;
+        }
+        f32x2_t sg = pair(g1, 0.f), sgh = pair(g1 * h1, 0.f), kept_h[KEEP ? Q : 1], kept_g[KEEP ? Q : 1];
 #pragma unroll
         for (int k = 0; k < PACKS; ++k)
         {
-            Pack<T, VEC> x[1], g[1], wk[1] = {w[k]};
-            read_row<T, VEC, TPR>(x, at_x + k * TPR * 16, t, a.dim - k * TPR * VEC);
-            read_row<T, VEC, TPR>(g, at_g + k * TPR * 16, t, a.dim - k * TPR * VEC);
+            const int at = cut.head + (k * TPR + t) * VEC;
+            if (at >= cut.end)
+                continue;
+            const Pack<T, VEC> x[1] = {read_packet<T, VEC, ANY>(at_x, at)}, wk[1] = {w[k]};
+            const Pack<T, VEC> g[1] = {read_packet<T, VEC, ANY>(at_g, at)};
 #pragma unroll
             for (int q = 0; q < VEC / 2; ++q)
             {
@@ -400,8 +697,8 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
 #pragma unroll
             for (int k = 0; k < PACKS; ++k)
             {
-                const int64_t i = ((int64_t) k * TPR + t) * VEC;
-                if (i >= a.dim)
+                const int i = cut.head + (k * TPR + t) * VEC;
+                if (i >= cut.end)
                     continue;
                 Pack<T, VEC> o[1];
                 if constexpr (KEEP)
@@ -412,9 +709,8 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
                 }
                 else
                 {
-                    Pack<T, VEC> x[1], g[1], wk[1] = {w[k]};
-                    read_row<T, VEC, TPR>(x, at_x + k * TPR * 16, t, a.dim - k * TPR * VEC);
-                    read_row<T, VEC, TPR>(g, at_g + k * TPR * 16, t, a.dim - k * TPR * VEC);
+                    const Pack<T, VEC> x[1] = {read_packet<T, VEC, ANY>(at_x, i)}, wk[1] = {w[k]};
+                    const Pack<T, VEC> g[1] = {read_packet<T, VEC, ANY>(at_g, i)};
 #pragma unroll
                     for (int q = 0; q < VEC / 2; ++q)
                         set_lanes(o, q,
@@ -422,6 +718,8 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
                 }
                 store_pack<T, VEC>((T*) a.dx + row * a.dim + i, o[0]);
             }
+            if (one_more)
+                ((T*) a.dx)[row * a.dim + cut.mine] = from_f32<T>(fmaf(h1, c1, fmaf(g1, r, c0)));
         }
         if (!KEEP && !LATE)
         {
@@ -444,12 +742,30 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
 #pragma unroll
         for (int q = 0; q < Q; ++q)
             set_lanes(o, q, which ? db[q] : dw[q]);
+        auto put = [&](float* to) {
+            if constexpr (ANY)
+            {
+#pragma unroll
+                for (int k = 0; k < PACKS; ++k)
+                {
+                    const int i = cut.head + (k * TPR + t) * VEC;
+                    if (i < cut.end)
+#pragma unroll
+                        for (int c = 0; c < VEC; ++c)
+                            to[i + c] = o[k].v[c];
+                }
+                if (one_more)
+                    to[cut.mine] = which ? db1 : dw1;
+            }
+            else
+                store_row<float, VEC, TPR>(o, to, t, a.dim);
+        };
         if constexpr (GROUPS == 1)
-            store_row<float, VEC, TPR>(o, part + which * a.dim, t, a.dim);
+            put(part + which * a.dim);
         else
         {
             __syncthreads();
-            store_row<float, VEC, TPR>(o, sums + group * a.dim, t, a.dim);
+            put(sums + group * a.dim);
             __syncthreads();
             for (int i = threadIdx.x; i < a.dim; i += 256)
             {
@@ -464,7 +780,7 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Backward without 16-byte boundaries, and of short rows: as norm_bwd_ring_kernel, but the next row is fetched into
+// Backward of short rows, and of few rows off 16-byte boundaries: as norm_bwd_ring_kernel, but the next row is fetched into
 // registers while the current one is reduced.  Up to TPR = 32 a warp takes 32 / TPR neighbouring rows at a time.
 // ------------------------------------------------------------------------------------------------------------------
 template <int TPR, int COLUMNS>
@@ -511,7 +827,7 @@ __global__ void __launch_bounds__(BwdShape<TPR, PACKS * VEC>::kThreads, BwdShape
     {
         if (!AHEAD)
             fetch(row);
-        const float r = rstd;
+        const float r = rstd, mean = mu;
         const f32x2_t m2 = pair(mu, mu), r2 = pair(r, r);
         f32x2_t h[Q], gw[Q], sg = zero, sgh = zero;
         Pack<T, VEC> w[PACKS];
@@ -533,6 +849,21 @@ __global__ void __launch_bounds__(BwdShape<TPR, PACKS * VEC>::kThreads, BwdShape
             fetch(row + stride);
         if (!a.dx)
             continue;
+        if (!(fabsf(mean * r) <= FLT_MAX))   // outside the row h is not finite, and 0 h no 0
+        {
+            sgh = zero;
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+            {
+                float h0, h1, g0, g1;
+                unpair(h[q], h0, h1);
+                unpair(gw[q], g0, g1);
+                const int i = 2 * q, j = 2 * q + 1;
+                const bool in0 = ((int64_t) (i / VEC) * TPR + t) * VEC + i % VEC < a.dim;
+                const bool in1 = j < N && ((int64_t) (j / VEC) * TPR + t) * VEC + j % VEC < a.dim;
+                sgh            = add2(sgh, pair(in0 ? g0 * h0 : 0.f, in1 ? g1 * h1 : 0.f));
+            }
+        }
         const float2 s = row_sum2<TPR>(lane_sum(sg), lane_sum(sgh), red[slot]);
         // dx = r gw - r mean(g) - h r mean(g h)
         const float c0 = -r * (s.x / (float) a.dim), c1 = -r * (s.y / (float) a.dim);
@@ -762,6 +1093,25 @@ int with_even_shape(int64_t packets, F&& f)
     AQ_SHAPE(512, 8)
     return AQ_ERR_TOO_LARGE;
 }
+// many rows of packets off 16-byte boundaries
+template <typename F>
+int with_any_shape(int64_t packets, F&& f)
+{
+    constexpr int MAX_PACKS = 4;
+    AQ_SHAPE(32, 1)
+    AQ_SHAPE(32, 2)
+    AQ_SHAPE(32, 4)
+    AQ_SHAPE(128, 2)
+    AQ_SHAPE(128, 3)
+    AQ_SHAPE(128, 4)
+    AQ_SHAPE(320, 2)
+    AQ_SHAPE(384, 2)
+    AQ_SHAPE(256, 4)
+    AQ_SHAPE(320, 4)
+    AQ_SHAPE(384, 4)
+    AQ_SHAPE(512, 4)
+    return AQ_ERR_TOO_LARGE;
+}
 // short rows of packets with sums: at most 16 columns per thread
 template <int MAX_PACKS, typename F>
 int with_short_shape(int64_t packets, F&& f)
@@ -777,7 +1127,7 @@ int with_short_shape(int64_t packets, F&& f)
 }
 // the backward ring: 16 columns per thread where the row's length allows; a warp takes up to
 // 768 elements of 16 bits or 512 of 32 alone
-template <typename T, typename F>
+template <typename T, bool ANY, typename F>
 int with_sums_shape(int64_t packets, F&& f)
 {
     constexpr int MAX_PACKS = 8;
@@ -788,7 +1138,15 @@ int with_sums_shape(int64_t packets, F&& f)
         AQ_SHAPE(32, 3)
         AQ_SHAPE(128, 1)
         AQ_SHAPE(128, 2)
+        if constexpr (ANY)
+        {
+            AQ_SHAPE(192, 2)
+        }
         AQ_SHAPE(256, 2)
+        if constexpr (ANY)
+        {
+            AQ_SHAPE(320, 2)
+        }
         AQ_SHAPE(512, 2)
         AQ_SHAPE(512, 3)
         AQ_SHAPE(512, 4)
@@ -797,7 +1155,15 @@ int with_sums_shape(int64_t packets, F&& f)
     {
         AQ_SHAPE(32, 4)
         AQ_SHAPE(128, 4)
+        if constexpr (ANY)
+        {
+            AQ_SHAPE(192, 4)
+        }
         AQ_SHAPE(256, 4)
+        if constexpr (ANY)
+        {
+            AQ_SHAPE(320, 4)
+        }
         AQ_SHAPE(512, 4)
         AQ_SHAPE(512, 6)
         AQ_SHAPE(512, 8)
@@ -819,11 +1185,11 @@ int ring_stages(int64_t stage_bytes, int groups, int& ctas)
     return 0;
 }
 
-template <typename Args, typename Kernel>
-int launch_ring(Kernel kernel, const Args& a, int stages, int groups, int matrices, int64_t elem, int64_t grid, int threads,
+template <typename Kernel>
+int launch_ring(Kernel kernel, const LayerNormGradArgs& a, int stages, int groups, int64_t stage_bytes, int64_t grid, int threads,
                 cudaStream_t st)
 {
-    const int64_t smem = (int64_t) groups * stages * (matrices * a.dim * elem + 8);
+    const int64_t smem = groups * stages * (stage_bytes + 8);
     cudaError_t e      = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
     if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3((unsigned) grid), threads, (size_t) smem, st, a, stages);
@@ -840,6 +1206,15 @@ bool wide_rows(const void* a, int64_t lda, const void* b, int64_t ldb, const voi
     return dim % W == 0 && fits(a, lda) && fits(b, ldb) && fits(w, W) && fits(bias, W) && fits(out, dim);
 }
 
+// Rows off 16-byte boundaries in packets all the same (see Cut), where that pays, forward and backward: 1024 x 4097 bf16
+// 12 + 18 us against 15 + 24 us element by element, 5000 x 513 9.4 + 9.8 against 10.2 + 12.3, but 297 x 1001 5.9 + 5.8
+// against 4.2 + 3.6 (a group's first row waits for its part of w and b), and 100000 x 65 31 + 58 against 22 + 34.
+template <typename T>
+bool any_rows(int64_t rows, int64_t dim, int64_t ld, int64_t ld2)
+{
+    constexpr int64_t W = 32 / (int) sizeof(T);
+    return rows >= 5 * kNumSMs && dim >= 512 && ld >= W && ld2 >= W;
+}
 template <typename T, int VEC>
 int norm_fwd_v(const LayerNormArgs& a, cudaStream_t st)
 {
@@ -864,7 +1239,28 @@ template <typename T>
 int norm_fwd_t(const LayerNormArgs& a, cudaStream_t st)
 {
     const bool wide = wide_rows<T>(a.x, a.ldx, nullptr, 0, a.w, a.b, a.y, a.dim);
-    const int rc    = wide ? norm_fwd_v<T, 16 / (int) sizeof(T)>(a, st) : norm_fwd_v<T, 1>(a, st);
+    int rc          = AQ_ERR_TOO_LARGE;
+    if (wide)
+        rc = norm_fwd_v<T, 16 / (int) sizeof(T)>(a, st);
+    else if (any_rows<T>(a.rows, a.dim, a.ldx, a.ldx))
+        rc = with_any_shape(a.dim / (16 / (int) sizeof(T)), [&](auto tpr, auto packs) {
+            using S      = AnyShape<decltype(tpr)::value, decltype(packs)::value>;
+            int64_t grid = (a.rows + S::kRows - 1) / S::kRows;
+            if (grid > S::kCtas * kNumSMs)
+            {
+                constexpr int VEC = 16 / (int) sizeof(T);
+                grid              = S::kCtas * kNumSMs;
+                grid -= grid * S::kRows % VEC;   // rows of a group a multiple of 16 bytes apart
+            }
+            const cudaError_t e = launch_pdl(norm_fwd_any_kernel<T, decltype(tpr)::value, decltype(packs)::value>,
+                                             dim3((unsigned) grid), S::kThreads, 0, st, a);
+            note_launch();
+            return e == cudaSuccess ? AQ_OK : cuda_fail(e);
+        });
+    if (rc != AQ_ERR_TOO_LARGE)
+        return rc;
+    if (!wide)
+        rc = norm_fwd_v<T, 1>(a, st);
     if (rc != AQ_ERR_TOO_LARGE)
         return rc;
     const int64_t grid  = a.rows < 8 * kNumSMs ? a.rows : 8 * kNumSMs;
@@ -876,24 +1272,27 @@ int norm_fwd_t(const LayerNormArgs& a, cudaStream_t st)
 // Most CTAs of the backward kernels, each with one row of partial sums: what the registers let reside anyway.
 int64_t bwd_ctas(int64_t rows, int64_t dim)
 {
-    const int64_t n = kNumSMs * (dim <= 1024 ? 8 : dim <= 2048 ? 4 : dim <= 4096 ? 2 : 1);
+    const int64_t n = kNumSMs * (dim <= 1024 ? 8 : dim <= 2048 ? 4 : dim <= 8192 ? 2 : 1);
     return rows < 1 ? 1 : rows < n ? rows : n;
 }
 
-template <typename T>
-int norm_bwd_wide(const LayerNormGradArgs& a, cudaStream_t st)
+template <typename T, bool ANY>
+int norm_bwd_ring(const LayerNormGradArgs& a, cudaStream_t st)
 {
     constexpr int VEC = 16 / (int) sizeof(T);
-    return with_sums_shape<T>(a.dim / VEC, [&](auto tpr, auto packs) -> int {
+    return with_sums_shape<T, ANY>(a.dim / VEC, [&](auto tpr, auto packs) -> int {
         constexpr int TPR = decltype(tpr)::value, PACKS = decltype(packs)::value;
-        using S     = RingShape<TPR>;
-        int ctas    = ctas_for(BwdColumns<T, PACKS>::kRegs, S::kThreads);
-        const int n = ring_stages(2 * a.dim * (int64_t) sizeof(T), S::kGroups, ctas);
+        using S             = RingShape<TPR>;
+        const int64_t bytes = 2 * ring_row_bytes(a.dim * (int64_t) sizeof(T), ANY);
+        int ctas            = ctas_for(BwdColumns<T, PACKS>::kRegs, S::kThreads);
+        const int n         = ring_stages(bytes, S::kGroups, ctas);
         if (n == 0)
             return AQ_ERR_TOO_LARGE;
         const int64_t most = bwd_ctas((a.rows + S::kGroups - 1) / S::kGroups, a.dim);
-        const int64_t grid = most < (int64_t) ctas * kNumSMs ? most : (int64_t) ctas * kNumSMs;
-        const int rc = launch_ring(norm_bwd_ring_kernel<T, TPR, PACKS>, a, n, S::kGroups, 2, sizeof(T), grid, S::kThreads, st);
+        int64_t grid       = most < (int64_t) ctas * kNumSMs ? most : (int64_t) ctas * kNumSMs;
+        if (ANY && grid * S::kGroups < a.rows)   // rows of a group a multiple of 16 bytes apart
+            grid -= grid * S::kGroups % VEC;
+        const int rc = launch_ring(norm_bwd_ring_kernel<T, TPR, PACKS, ANY>, a, n, S::kGroups, bytes, grid, S::kThreads, st);
         if (rc != AQ_OK || !a.part)
             return rc;
         return fold_columns(a.part, grid, 2 * a.dim, a.dim, a.dw, a.db, a.dtype, st);
@@ -934,9 +1333,20 @@ template <typename T>
 int norm_bwd_t(const LayerNormGradArgs& a, cudaStream_t st)
 {
     const bool wide = wide_rows<T>(a.x, a.ldx, a.dy, a.lddy, a.w, nullptr, a.dx, a.dim);
-    int rc          = wide ? norm_bwd_registers<T, 16 / (int) sizeof(T)>(a, st) : norm_bwd_registers<T, 1>(a, st);
-    if (rc == AQ_ERR_TOO_LARGE && wide)
-        rc = norm_bwd_wide<T>(a, st);
+    int rc          = AQ_ERR_TOO_LARGE;
+    if (wide)
+    {
+        rc = norm_bwd_registers<T, 16 / (int) sizeof(T)>(a, st);
+        if (rc == AQ_ERR_TOO_LARGE)
+            rc = norm_bwd_ring<T, false>(a, st);
+    }
+    else
+    {
+        if (any_rows<T>(a.rows, a.dim, a.ldx, a.lddy))
+            rc = norm_bwd_ring<T, true>(a, st);
+        if (rc == AQ_ERR_TOO_LARGE)
+            rc = norm_bwd_registers<T, 1>(a, st);
+    }
     if (rc != AQ_ERR_TOO_LARGE)
         return rc;
     if (a.dx)

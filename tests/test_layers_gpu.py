@@ -358,6 +358,52 @@ def test_norm_layouts(cuda, dtype, dim):
     assert bias_only.grad.shape == shape
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("dim", [65, 300, 512, 513, 519, 777, 1001, 1537, 2051, 4096, 4099, 5001, 6145, 8193, 12001, 16391, 20001])
+def test_norm_rows_off_boundaries(cuda, dtype, dim):
+    """Many rows of odd lengths and pitches, each tensor with its own alignment; what lies between the rows is NaN."""
+    g = _gen(61 + dim)
+    rows = 745 + dim % 5
+
+    def inside(start, pad, **kw):
+        wide = torch.full((rows, dim + start + pad), float("nan"), device=cuda, dtype=dtype)
+        wide[:, start:start + dim] = _randn(g, rows, dim, dtype=dtype, **kw)
+        return wide[:, start:start + dim]
+
+    w, b = _randn(g, dim + 1, dtype=dtype, shift=1.0)[1:], _randn(g, dim + 3, dtype=dtype)[3:]
+    for k, (x, dy) in enumerate(((inside(0, 0, shift=0.5), inside(0, 0)), (inside(3, 0), inside(0, 1)),
+                                 (inside(1, 8), inside(8, 7)))):
+        _check_norm(x, (dim,), w if k != 1 else None, b if k != 2 else None, 1e-5, dy, f"{rows}x{dim} layout {k}")
+    from aimet_b200.v2.nn import layer_norm
+    x, dy = inside(5, 2).requires_grad_(True), inside(0, 3)
+    ref = norm_ref(x, w, b, 1e-5, dy)
+    for name, leaf, args in (("dx", x, (x, w, b)), ("dw", w.requires_grad_(True), (x.detach(), w, b)),
+                             ("db", b.requires_grad_(True), (x.detach(), w.detach(), b))):
+        y = layer_norm(args[0], dim, args[1], args[2], 1e-5)
+        assert_within(torch.autograd.grad(y, leaf, dy)[0], ref[name], name + " alone")
+
+
+@pytest.mark.parametrize("dtype", DTYPES[::2], ids=str)
+@pytest.mark.parametrize("rows,dim", [(5, 40), (5, 65), (5, 1000), (800, 40), (800, 65), (800, 1000), (800, 1001)])
+def test_norm_large_constant_rows(cuda, dtype, rows, dim):
+    """mean rstd passes float32's range, h does not: 2^117 and its sums over a row are exact, so h is 0 and
+    dx = rstd (dy - mean dy)."""
+    from aimet_b200.v2.nn import layer_norm
+    g = _gen(67)
+    x = torch.full((rows, dim), 2.0 ** 117, device=cuda, dtype=dtype, requires_grad=True)
+    dy = _randn(g, rows, dim, dtype=dtype)
+    y = layer_norm(x, dim, None, None, 1e-12)
+    assert not bool(y.detach().any())
+    (dx,) = torch.autograd.grad(y, x, dy)
+    d = dy.double()
+    mean, size = d.mean(1, keepdim=True), d.abs().mean(1, keepdim=True)
+    want = 1e6 * (d - mean)
+    # the sum of dim terms and its quotient; the products with rstd and the difference; rstd's root and quotient; the result
+    e = 1e6 * ((dim + 8) * 2.0 ** -24 * size + 3 * 2.0 ** -24 * (d.abs() + size)) + 4 * 2.0 ** -24 * want.abs()
+    u = torch.finfo(dtype).eps / 2
+    assert bool(((dx.double() - want).abs() <= e * (1 + u) + u * want.abs()).all())
+
+
 @pytest.mark.parametrize("dim", [96, 1024, 1537, 11008, 40000])
 def test_norm_mean_far_from_zero(cuda, dim):
     """|mean| a thousand times the spread: the variance is not formed as a difference of two large numbers."""
@@ -379,17 +425,21 @@ def test_norm_constant_rows(cuda, dtype, dim):
     assert bool((dx == 0).all())
 
 
-@pytest.mark.parametrize("dim", [64, 1000, 4096, 40000])
-def test_norm_inf_and_nan_stay_in_their_rows(cuda, dim):
+@pytest.mark.parametrize("rows,dim", [(40, 64), (40, 1000), (40, 4096), (40, 40000), (800, 65), (800, 1001), (800, 4101)])
+def test_norm_inf_and_nan_stay_in_their_rows(cuda, rows, dim):
     from aimet_b200.v2.nn import layer_norm
     g = _gen(47)
-    x = _randn(g, 40, dim, dtype=torch.bfloat16)
+    x = _randn(g, rows, dim, dtype=torch.bfloat16)
     clean = layer_norm(x, dim)
     bad = x.clone()
     bad[3, 5], bad[17, dim - 1] = float("nan"), float("inf")
     y = layer_norm(bad, dim)
-    keep = [i for i in range(40) if i not in (3, 17)]
+    keep = [i for i in range(rows) if i not in (3, 17)]
     assert torch.equal(y[keep], clean[keep]) and bool(y[3].isnan().all()) and bool(y[17].isnan().all())
+    bad.requires_grad_(True)
+    dy = _randn(g, rows, dim, dtype=torch.bfloat16)
+    (dx,) = torch.autograd.grad(layer_norm(bad, dim), bad, dy)
+    assert bool(dx[keep].isfinite().all()) and not bool(dx[[3, 17]].isfinite().any())
 
 
 def test_norm_empty(cuda):

@@ -26,6 +26,7 @@ NVCC_FLAGS = [
     "-fmad=false",
     "-Xcompiler", "-fPIC,-O2,-ffp-contract=off",
     "-shared",
+    "--threads", "0",   # the sources side by side
 ]
 
 

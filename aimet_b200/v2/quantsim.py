@@ -208,11 +208,17 @@ def fuse_layers(gm: fx.GraphModule) -> int:
             continue
         last = node
         kwargs = dict(node.kwargs)
+
+        def quiet(user):
+            """The fused layer runs, and reads its input, at ``user``: nothing may be written in place on the way there,
+            except by the activation that has been taken in."""
+            return not any(order[node] < w < order[user] and w != order[last] for w in writers)
+
         user = _single_user(last)
         if "residual" not in kwargs and "activation" not in kwargs and user is not None and \
                 user.args and user.args[0] is last:
             name = _activation_name(user, mods)
-            if name is not None:
+            if name is not None and quiet(user):
                 kwargs["activation"] = name
                 last = user
                 user = _single_user(last)
@@ -220,10 +226,8 @@ def fuse_layers(gm: fx.GraphModule) -> int:
                 len(user.args) == 2 and not user.kwargs:
             left, right = user.args
             other = right if left is last else left
-            # x += linear(...) writes to x; anything written in place in between could change what the layer reads
-            mine = (order[last],) if last is not node else ()
-            quiet = not any(order[node] < w < order[user] and w not in mine for w in writers)
-            if isinstance(other, fx.Node) and other is not last and quiet and \
+            # x += linear(...) writes to x
+            if isinstance(other, fx.Node) and other is not last and quiet(user) and \
                     (user.target is not operator.iadd or left is last):
                 kwargs["residual"] = other
                 last = user

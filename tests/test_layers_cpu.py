@@ -203,3 +203,65 @@ def test_layer_norm_module_shares_parameters():
     assert new.state_dict().keys() == old.state_dict().keys()
     bare = LayerNorm.from_module(nn.LayerNorm(5, elementwise_affine=False))
     assert bare.weight is None and bare.bias is None
+
+
+def _mul_between(s, x):
+    h = x * 1.0
+    y = s.a(h)
+    h.mul_(2.0)
+    return F.relu(y)
+
+
+def _relu_between(s, x):
+    h = x * 1.0
+    y = s.a(h)
+    h.relu_()
+    return F.gelu(y) + s.b(h)
+
+
+def _module_between(s, x):
+    h = s.n(x)
+    y = s.a(h)
+    g = s.r(h)
+    return F.silu(y) * g
+
+
+def _function_between(s, x):
+    h = x * 1.0
+    y = s.a(h)
+    F.relu(h, inplace=True)
+    return torch.relu(y)
+
+
+def _dropout_between(s, x):
+    h = x * 1.0
+    y = s.a(h)
+    F.dropout(h, 1.0, True, inplace=True)
+    return s.g(y)
+
+
+def _between_activation_and_addition(s, x):
+    h = x * 1.0
+    y = F.relu(s.a(h))
+    h.mul_(2.0)
+    return y + x
+
+
+@pytest.mark.parametrize("fn,mods,want", [
+    (_mul_between, {}, [("linear", None, False)]),
+    (_relu_between, {}, None),
+    (_module_between, {"r": nn.ReLU(inplace=True)}, [("layer_norm",), ("linear", None, False)]),
+    (_function_between, {}, [("linear", None, False)]),
+    (_dropout_between, {"g": nn.GELU()}, [("linear", None, False)]),
+    (_between_activation_and_addition, {}, [("linear", "relu", False)]),
+])
+def test_fuse_layers_reads_the_input_before_it_is_written(on_torch, fn, mods, want):
+    """The layer's input is written in place before the activation (or the addition) is reached."""
+    torch.manual_seed(0)
+    net = _Net(fn, **mods).eval()
+    x = torch.randn(5, 8)
+    expect = net(x.clone())
+    sim, _ = _fused(net)
+    assert torch.allclose(sim.model(x.clone()), expect, atol=1e-6)
+    if want is not None:
+        assert on_torch == want

@@ -63,10 +63,9 @@ class QuantizedLayer(nn.Module):
 
 class QuantizedLinear(QuantizedLayer):
     """A linear layer on :func:`aimet_b200.v2.nn.linear`: the activation and the addition that follow it in the traced
-    graph arrive as arguments and run in the product's epilogue.  ``into``: the addition was ``y += residual``, whose
-    result keeps the layer's shape and dtype."""
+    graph arrive as arguments and run in the product's epilogue."""
 
-    def forward(self, x, residual=None, activation=None, into=False):   # pylint: disable=arguments-differ
+    def forward(self, x, residual=None, activation=None):   # pylint: disable=arguments-differ
         wq = self.param_quantizers["weight"]
         weight = self.layer.weight if wq is None else wq(self.layer.weight)
         if residual is None:
@@ -74,11 +73,7 @@ class QuantizedLinear(QuantizedLayer):
         if isinstance(residual, torch.Tensor) and residual.shape == x.shape[:-1] + weight.shape[:1] and \
                 residual.dtype == x.dtype and residual.device == x.device:
             return qnn.linear(x, weight, self.layer.bias, activation, residual)
-        y = qnn.linear(x, weight, self.layer.bias, activation)
-        if into:   # broadcast, promoted or refused by torch
-            y += residual
-            return y
-        return y + residual
+        return qnn.linear(x, weight, self.layer.bias, activation) + residual   # broadcast or promoted by torch
 
 
 @torch.no_grad()
@@ -235,8 +230,6 @@ def fuse_layers(gm: fx.GraphModule) -> int:
             if isinstance(other, fx.Node) and other is not last and quiet(user) and \
                     (user.target is not operator.iadd or left is last):
                 kwargs["residual"] = other
-                if user.target is operator.iadd:
-                    kwargs["into"] = True
                 last = user
         if last is node:
             continue

@@ -265,32 +265,3 @@ def test_fuse_layers_reads_the_input_before_it_is_written(on_torch, fn, mods, wa
     assert torch.allclose(sim.model(x.clone()), expect, atol=1e-6)
     if want is not None:
         assert on_torch == want
-
-
-def test_fuse_layers_keeps_what_an_in_place_addition_returns(on_torch):
-    """y += r stays y: its dtype and shape are the layer's, and an r that does not fit into it is refused."""
-    def into(s, x, r):
-        y = s.a(x)
-        y += r
-        return y
-
-    class Net(nn.Module):
-        def __init__(self):
-            super().__init__()
-            self.a = nn.Linear(8, 8)
-
-        def forward(self, x, r):
-            return into(self, x, r)
-
-    torch.manual_seed(0)
-    net = Net().eval()
-    x = torch.randn(5, 8)
-    sim, changed = _fused(net)
-    for r in (torch.randn(5, 8), torch.randn(5, 8, dtype=torch.float64), torch.randn(8), torch.arange(8)):
-        want = net(x, r)
-        got = sim.model(x, r)
-        assert got.dtype == want.dtype and got.shape == want.shape and torch.allclose(got, want, atol=1e-6)
-    assert on_torch == [("linear", None, True)] + [("linear", None, False)] * 3
-    for call in (net, sim.model):
-        with pytest.raises(RuntimeError):
-            call(x, torch.randn(3, 5, 8))

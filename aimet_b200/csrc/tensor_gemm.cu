@@ -742,10 +742,23 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int64_
     const cuuint64_t pitch[1]   = {(cuuint64_t) ld * 2};
     const cuuint32_t box[2]     = {(cuuint32_t) kBlockK, (cuuint32_t) box_rows};
     const cuuint32_t strides[2] = {1, 1};
-    const CUresult r =
-        fn(map, dtype == AQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
-           dims, pitch, box, strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return fn(map, dtype == AQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
+                  dims, pitch, box, strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED)
+    {
+        // the first CUDA call of this host thread: the driver has no context for it until the runtime binds one
+        int dev       = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess)
+            e = cudaSetDevice(dev);
+        if (e != cudaSuccess)
+            return cuda_fail(e);
+        r = encode();
+    }
     return r == CUDA_SUCCESS ? AQ_OK : AQ_ERR_INVALID_ARG;
 }
 

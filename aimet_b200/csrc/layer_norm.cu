@@ -1172,13 +1172,14 @@ int with_sums_shape(int64_t packets, F&& f)
 }
 #undef AQ_SHAPE
 
+constexpr int kRingBudget = 208 * 1024;   // shared memory of an SM for the rings of its CTAs
+
 // Stages of a ring: as many as fit with `ctas` CTAs on an SM (or fewer CTAs), 2 to 6; 0 when two do not fit.
 int ring_stages(int64_t stage_bytes, int groups, int& ctas)
 {
-    constexpr int64_t kBudget = 208 * 1024;
     for (; ctas >= 1; --ctas)
     {
-        const int64_t n = kBudget / ctas / (stage_bytes * groups + 8 * groups);
+        const int64_t n = kRingBudget / ctas / (stage_bytes * groups + 8 * groups);
         if (n >= (ctas > 1 ? 3 : 2))
             return (int) (n < 6 ? n : 6);
     }
@@ -1190,7 +1191,8 @@ int launch_ring(Kernel kernel, const LayerNormGradArgs& a, int stages, int group
                 cudaStream_t st)
 {
     const int64_t smem = groups * stages * (stage_bytes + 8);
-    cudaError_t e      = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
+    // the same limit on every call: it belongs to the kernel, and another host thread may be about to launch with more
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBudget);
     if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3((unsigned) grid), threads, (size_t) smem, st, a, stages);
     note_launch();

@@ -798,13 +798,15 @@ int wide_access(const GemmArgs& a)
     return 0;
 }
 
+// `most`: the most shared memory that any call of the kernel asks for.  The limit belongs to the kernel, not to the launch,
+// so every call sets it to the same value: a smaller one would refuse the launch that another host thread is about to make.
 template <typename Kernel>
-int launch(Kernel kernel, int64_t grid, int cluster, int threads, int smem, cudaStream_t st, const CUtensorMap& ma,
+int launch(Kernel kernel, int64_t grid, int cluster, int threads, int smem, int most, cudaStream_t st, const CUtensorMap& ma,
            const CUtensorMap& mb, const TcArgs& p)
 {
     if (grid > 0x7fffffff)
         return AQ_ERR_TOO_LARGE;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess)
         e = launch_cluster(kernel, (unsigned) grid, cluster, threads, smem, st, ma, mb, p);
     note_launch();
@@ -830,8 +832,8 @@ int run_pair(const GemmArgs& a, cudaStream_t st)
         return AQ_ERR_TOO_LARGE;
     const int64_t pairs = tiles < kNumSMs / 2 ? tiles : kNumSMs / 2;
     return with_activation(a.act, [&](auto act) {
-        return launch(pair_kernel<T, BN, decltype(act)::value>, 2 * pairs, 2, 128 + 32 * kPairWarps, PairShape<BN>::kSmem, st, ma,
-                      mb, p);
+        return launch(pair_kernel<T, BN, decltype(act)::value>, 2 * pairs, 2, 128 + 32 * kPairWarps, PairShape<BN>::kSmem,
+                      PairShape<BN>::kSmem, st, ma, mb, p);
     });
 }
 
@@ -853,7 +855,7 @@ int run_slim(const GemmArgs& a, int splits, cudaStream_t st)
     p.idesc            = instruction_desc(a.dtype == AQ_BF16, a.b_kmajor, a.a_kmajor, 128, BN);
     const int64_t ctas = (int64_t) p.tiles_i * p.tiles_j * splits;
     p.stages           = ctas <= kNumSMs ? S::kDeep : S::kShallow;
-    return launch(slim_kernel<T, BN>, ctas, splits, 192, S::smem(p.stages), st, ma, mb, p);
+    return launch(slim_kernel<T, BN>, ctas, splits, 192, S::smem(p.stages), S::smem(S::kDeep), st, ma, mb, p);
 }
 
 // Clusters of `splits` CTAs of slim_kernel that the current device holds at once (a cluster lives inside one GPC, so this
@@ -868,7 +870,7 @@ int resident_clusters(int splits)
     int n = known[dev][splits].load(std::memory_order_relaxed);
     if (n == 0)
     {
-        cudaFuncSetAttribute(slim_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SlimShape<BN>::smem(SlimShape<BN>::kShallow));
+        cudaFuncSetAttribute(slim_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SlimShape<BN>::smem(SlimShape<BN>::kDeep));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim            = dim3(splits);
         cfg.blockDim           = dim3(192);

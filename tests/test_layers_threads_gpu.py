@@ -43,3 +43,77 @@ def test_first_cuda_call_of_a_host_thread(cuda, m):
         torch.cuda.synchronize()
         assert torch.equal(y, want)
     assert torch.equal(_in_thread(lambda: linear(x, w)), want)
+
+
+def _race(jobs, calls):
+    """Every job on a thread and a stream of its own; the foreign calls release the interpreter's lock."""
+    gate = threading.Barrier(len(jobs))
+    failed = []
+
+    def work(job):
+        stream = torch.cuda.Stream()
+        gate.wait()
+        for i in range(calls):
+            rc = job(stream.cuda_stream)
+            if rc:
+                failed.append((i, rc))
+                break
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(job,)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return failed
+
+
+def _check_race(jobs, outs):
+    stream = torch.cuda.current_stream().cuda_stream
+    want = []
+    for job, out in zip(jobs, outs):
+        assert job(stream) == 0
+        want.append(out.clone())
+    torch.cuda.synchronize()
+    assert _race(jobs, 20000) == []
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("m", [64, 100])
+def test_products_from_two_threads(cuda, m):
+    """One kernel, called with its deep pipeline by one thread and with its shallow one by the other."""
+    from aimet_b200._lib import lib
+    g = torch.Generator(device="cuda").manual_seed(89)
+    jobs, outs = [], []
+    for n, k in ((512, 512), (25600, 64)):
+        x = torch.randn(m, k, device=cuda, generator=g).bfloat16()
+        w = torch.randn(n, k, device=cuda, generator=g).bfloat16()
+        y = torch.empty(m, n, device=cuda, dtype=torch.bfloat16)
+
+        def job(stream, x=x, w=w, n=n, k=k, y=y):
+            return lib.aq_linear_forward(x.data_ptr(), k, w.data_ptr(), k, None, None, 0, y.data_ptr(), n, None, 0, 2, m, n, k, 0,
+                                         stream)
+
+        jobs.append(job)
+        outs.append(y)
+    _check_race(jobs, outs)
+
+
+def test_norm_backward_from_two_threads(cuda):
+    """One kernel on rows of different lengths."""
+    from aimet_b200._lib import lib
+    g = torch.Generator(device="cuda").manual_seed(97)
+    jobs, outs = [], []
+    for rows, dim in ((16, 2064), (16, 4096)):
+        x, dy = (torch.randn(rows, dim, device=cuda, generator=g).bfloat16() for _ in range(2))
+        mean, rstd = x.float().mean(1).contiguous(), x.float().var(1, unbiased=False).rsqrt().contiguous()
+        dx = torch.empty(rows, dim, device=cuda, dtype=torch.bfloat16)
+
+        def job(stream, x=x, dy=dy, mean=mean, rstd=rstd, rows=rows, dim=dim, dx=dx):
+            return lib.aq_layer_norm_backward(x.data_ptr(), dim, dy.data_ptr(), dim, None, mean.data_ptr(), rstd.data_ptr(),
+                                              dx.data_ptr(), None, None, 2, rows, dim, None, 0, stream)
+
+        jobs.append(job)
+        outs.append(dx)
+    _check_race(jobs, outs)

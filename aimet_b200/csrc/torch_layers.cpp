@@ -3,6 +3,7 @@
 // forward and backward of a linear layer, 90 of them for the two crossings between autograd's engine and Python.
 //
 // The C entry points come from the library that the package has loaded (bind()); nothing is linked against it.
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -89,6 +90,16 @@ void check_operand(const Tensor& t, const Tensor& like, at::IntArrayRef shape, c
     TORCH_CHECK(t.scalar_type() == like.scalar_type(), "aimet_b200: ", name, " is ", t.scalar_type(), ", the input is ",
                 like.scalar_type());
     TORCH_CHECK(t.device() == like.device(), "aimet_b200: tensors on different devices (", like.device(), " vs ", t.device(), ")");
+}
+
+// The kernels know nothing of tangents, and a result without one would be taken for a constant.
+void check_tangents(std::initializer_list<const Tensor*> tensors)
+{
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        return;
+    for (const Tensor* t : tensors)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(),
+                    "aimet_b200: forward-mode derivatives are not provided for linear and layer_norm");
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> tensors)
@@ -241,6 +252,7 @@ struct Linear : torch::autograd::Function<Linear>
 
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
+        check_tangents({&grads[0]});
         const bool create_graph = at::GradMode::is_enabled();
         variable_list out(5);
         {
@@ -307,6 +319,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
               const std::optional<Tensor>& residual_arg)
 {
     const Tensor bias = bias_arg.value_or(Tensor()), residual = residual_arg.value_or(Tensor());
+    check_tangents({&x, &weight, &bias, &residual});
     check_input(x);
     TORCH_CHECK(weight.dim() == 2 && x.dim() >= 1 && weight.numel() > 0 && x.size(-1) == weight.size(1),
                 "aimet_b200: cannot apply a weight of shape ", weight.sizes(), " to an input of shape ", x.sizes());
@@ -372,6 +385,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm>
 
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
+        check_tangents({&grads[0]});
         const bool create_graph = at::GradMode::is_enabled();
         variable_list out(6);
         {
@@ -409,6 +423,7 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& shape, const std:
                   const std::optional<Tensor>& bias_arg, double eps)
 {
     const Tensor weight = weight_arg.value_or(Tensor()), bias = bias_arg.value_or(Tensor());
+    check_tangents({&x, &weight, &bias});
     check_input(x);
     int64_t dim = 1;
     for (int64_t s : shape)

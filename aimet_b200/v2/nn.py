@@ -12,7 +12,8 @@ that the two products of the backward pass read -- the tensor cores take operand
 copy would double the traffic.
 
 Quantized tensors (:mod:`aimet_b200.v2.qtensor`) count as the numbers they hold; results are plain tensors.  There is no
-CPU path: CPU tensors raise ``RuntimeError``.  Gradients of gradients are not provided.
+CPU path: CPU tensors raise ``RuntimeError``.  Gradients of gradients and forward-mode derivatives are not provided: both
+raise ``RuntimeError``.
 """
 from __future__ import annotations
 

@@ -265,3 +265,19 @@ def test_fuse_layers_reads_the_input_before_it_is_written(on_torch, fn, mods, wa
     assert torch.allclose(sim.model(x.clone()), expect, atol=1e-6)
     if want is not None:
         assert on_torch == want
+
+
+def test_forward_mode_tensors_are_refused():
+    """A result without a tangent would be taken for a constant."""
+    import torch.autograd.forward_ad as fwad
+    from aimet_b200.v2.nn import layer_norm, linear
+    x, w, b = torch.randn(2, 8), torch.randn(4, 8), torch.randn(4)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for call in (lambda: linear(dual(x), w), lambda: linear(x, dual(w)), lambda: linear(x, w, dual(b)),
+                     lambda: linear(x, w, residual=dual(torch.zeros(2, 4))), lambda: layer_norm(dual(x), 8),
+                     lambda: layer_norm(x, 8, dual(torch.ones(8))), lambda: layer_norm(x, 8, None, dual(torch.ones(8)))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+            linear(dual(x), w)   # no tangents are carried here, by torch's functions neither

@@ -112,12 +112,23 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors)
     return false;
 }
 
+// Memory that holds the tensor's numbers: a lazily negated view's memory holds the others.
+Tensor resolved(const Tensor& t)
+{
+    return t.defined() && t.is_neg() ? t.resolve_neg() : t;
+}
+// a vector as the kernels read it
+Tensor dense(const Tensor& t)
+{
+    return t.defined() ? resolved(t).contiguous() : t;
+}
+
 // `t` as a matrix of rows of `width` elements: a view where rows have unit stride and one pitch, else a copy
 Tensor rows_of(const Tensor& t, int64_t width)
 {
-    Tensor m = t;
+    Tensor m = resolved(t);
     if (t.dim() != 2 || t.size(1) != width)
-        m = t.reshape({t.numel() / width, width});
+        m = m.reshape({m.numel() / width, width});
     if ((width > 1 && m.stride(1) != 1) || (m.size(0) > 1 && m.stride(0) < width))
         m = m.contiguous();
     return m;
@@ -216,7 +227,7 @@ LinearParts linear_parts(const Tensor& x, const Tensor& weight, const Tensor& bi
         r.w = aligned_rows(r.w, on);
     }
     const Tensor res = residual.defined() ? rows_of(residual, n) : residual;
-    const Tensor b   = bias.defined() ? bias.contiguous() : bias;
+    const Tensor b   = dense(bias);
     auto shape       = x.sizes().vec();
     shape.back()     = n;
     r.y              = at::empty(shape, x.options());
@@ -348,8 +359,8 @@ NormParts norm_parts(const Tensor& x, int64_t dim, const Tensor& weight, const T
     On on(x);
     NormParts r;
     r.x                = rows_of(x, dim);
-    r.w                = weight.defined() ? weight.contiguous() : weight;
-    const Tensor b     = bias.defined() ? bias.contiguous() : bias;
+    r.w                = dense(weight);
+    const Tensor b     = dense(bias);
     const int64_t rows = r.x.size(0);
     r.y                = at::empty(x.sizes(), x.options());
     float* mean        = nullptr;

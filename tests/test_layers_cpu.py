@@ -281,3 +281,11 @@ def test_forward_mode_tensors_are_refused():
                 call()
         with torch.inference_mode(), pytest.raises(RuntimeError, match="must be a CUDA tensor"):
             linear(dual(x), w)   # no tangents are carried here, by torch's functions neither
+
+
+def test_rows_of_lazily_negated_tensors():
+    from aimet_b200.v2.nn import _layers
+    for t in (torch.randn(4, 8), torch.randn(2, 3, 8), torch.randn(8)):
+        n = torch._neg_view(t)
+        rows = _layers.rows_of(n, 8)
+        assert n.is_neg() and not rows.is_neg() and torch.equal(rows, -t.reshape(-1, 8))

@@ -687,7 +687,8 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
         float2 sum = row_sum2<TPR>(lane_sum(sg), lane_sum(sgh), red[slot]);
         if (!ok)
             sum.x = __int_as_float(0x7fffffff);
-        if ((KEEP || LATE) && t == 0 && row + ahead * stride < a.rows)
+        // not after a wait that ran out: the barrier's phase is still open, and a second arrival in it is not allowed
+        if ((KEEP || LATE) && t == 0 && ok && row + ahead * stride < a.rows)
             request(LATE ? (ring.stage == 0 ? stages - 1 : ring.stage - 1) : ring.stage, row + ahead * stride);
         if (a.dx)
         {
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
         if (!KEEP && !LATE)
         {
             __syncwarp();
-            if (t == 0 && row + ahead * stride < a.rows)
+            if (t == 0 && ok && row + ahead * stride < a.rows)
                 request(ring.stage, row + ahead * stride);
         }
         ring.advance();
@@ -733,6 +734,13 @@ __global__ void __launch_bounds__(RingShape<TPR>::kThreads, ctas_for(BwdColumns<
     tc::stuck_exit(&stuck_smem, &g_stuck);
     if (!a.part)
         return;
+    if (stuck_smem)   // rows that never arrived are in the sums
+    {
+        dw1 = db1 = __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            dw[q] = db[q] = pair(dw1, dw1);
+    }
     float* part = a.part + (int64_t) blockIdx.x * 2 * a.dim;
     float* sums = reinterpret_cast<float*>(ring_smem);   // [GROUPS][dim]: the ring is no longer needed
 #pragma unroll

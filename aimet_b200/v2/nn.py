@@ -17,6 +17,7 @@ raise ``RuntimeError``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.util
 import os
@@ -27,7 +28,7 @@ from torch import nn
 
 from .. import _lib
 
-__all__ = ["linear", "layer_norm", "LayerNorm", "ACTIVATIONS"]
+__all__ = ["linear", "layer_norm", "LayerNorm", "ACTIVATIONS", "wait_ran_out"]
 
 #: names the ``activation`` argument takes beside None
 ACTIVATIONS = {"relu": _lib.AQ_ACT_RELU, "gelu": _lib.AQ_ACT_GELU, "gelu_tanh": _lib.AQ_ACT_GELU_TANH,
@@ -79,6 +80,16 @@ def layer_norm(x: torch.Tensor, normalized_shape: Union[int, Sequence[int]], wei
     ``normalized_shape`` and the dtype of ``x``."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else normalized_shape
     return _layers.layer_norm(x, shape, weight, bias, eps)
+
+
+def wait_ran_out(device: Optional[torch.device] = None) -> bool:
+    """Whether a kernel of this module has given up waiting for its own copies or products on ``device`` (default: the
+    current one) since the library was loaded.  Every such wait is bounded (4 s); results that a wait was for hold NaN and
+    no call fails, so a program that meets NaN asks here.  Waits for the device."""
+    out = ctypes.c_int32(0)
+    with contextlib.nullcontext() if device is None else torch.cuda.device(device):
+        _lib.check(_lib.lib.aq_layers_stuck(ctypes.byref(out)), "aq_layers_stuck")
+    return bool(out.value)
 
 
 class LayerNorm(nn.LayerNorm):

@@ -289,3 +289,24 @@ def test_rows_of_lazily_negated_tensors():
         n = torch._neg_view(t)
         rows = _layers.rows_of(n, 8)
         assert n.is_neg() and not rows.is_neg() and torch.equal(rows, -t.reshape(-1, 8))
+
+
+def test_wait_ran_out_asks_the_library(monkeypatch):
+    """A library that answers as one whose wait has run out, as a sound one, and as one that cannot be asked."""
+    from aimet_b200.v2 import nn as qnn
+    real = qnn._lib.lib
+    answers = iter([(0, 1), (0, 0), (-3, 0)])
+
+    class Fake:
+        def aq_layers_stuck(self, out):
+            rc, out._obj.value = next(answers)
+            return rc
+
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+    monkeypatch.setattr(qnn._lib, "lib", Fake())
+    assert qnn.wait_ran_out() is True
+    assert qnn.wait_ran_out() is False
+    with pytest.raises(RuntimeError, match="aq_layers_stuck"):
+        qnn.wait_ran_out()

@@ -117,3 +117,8 @@ def test_norm_backward_from_two_threads(cuda):
         jobs.append(job)
         outs.append(dx)
     _check_race(jobs, outs)
+
+
+def test_no_wait_ran_out_here(cuda):
+    from aimet_b200.v2.nn import wait_ran_out
+    assert wait_ran_out() is False and wait_ran_out(cuda) is False

@@ -21,6 +21,7 @@ import contextlib
 import ctypes
 import importlib.util
 import os
+import threading
 from typing import Optional, Sequence, Union
 
 import torch
@@ -51,7 +52,21 @@ def _load():
     return module
 
 
-_layers = _load()
+_loading = threading.Lock()
+
+
+def __getattr__(name):
+    # `_layers` is loaded at its first use: a simulated model whose layers are never fused does not need it
+    if name != "_layers":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    with _loading:
+        if "_layers" not in globals():
+            globals()["_layers"] = _load()
+    return globals()["_layers"]
+
+
+def _native():
+    return globals().get("_layers") or __getattr__("_layers")
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -69,7 +84,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         act = ACTIVATIONS.get(activation)
         if act is None:
             raise ValueError(f"activation must be None or one of {tuple(ACTIVATIONS)}, got {activation!r}")
-    return _layers.linear(x, weight, bias, act, residual)
+    return _native().linear(x, weight, bias, act, residual)
 
 
 def layer_norm(x: torch.Tensor, normalized_shape: Union[int, Sequence[int]], weight: Optional[torch.Tensor] = None,
@@ -79,7 +94,7 @@ def layer_norm(x: torch.Tensor, normalized_shape: Union[int, Sequence[int]], wei
     ``x`` is float32, float16 or bfloat16 with any strides; ``weight`` and ``bias``, each optional, have the shape
     ``normalized_shape`` and the dtype of ``x``."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else normalized_shape
-    return _layers.layer_norm(x, shape, weight, bias, eps)
+    return _native().layer_norm(x, shape, weight, bias, eps)
 
 
 def wait_ran_out(device: Optional[torch.device] = None) -> bool:

@@ -310,3 +310,47 @@ def test_wait_ran_out_asks_the_library(monkeypatch):
     assert qnn.wait_ran_out() is False
     with pytest.raises(RuntimeError, match="aq_layers_stuck"):
         qnn.wait_ran_out()
+
+
+def test_simulated_models_do_not_need_the_torch_side():
+    """Without _torch_layers.so everything but the two layers works; these say what is missing."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import importlib.util
+real = importlib.util.spec_from_file_location
+def missing(name, *args, **kwargs):
+    if name == "_torch_layers":
+        raise ImportError("no torch side")
+    return real(name, *args, **kwargs)
+importlib.util.spec_from_file_location = missing
+import torch
+from aimet_b200.v2 import nn as qnn
+from aimet_b200.v2.quantsim import QuantizationSimModel
+sim = QuantizationSimModel(torch.nn.Sequential(torch.nn.Linear(4, 4), torch.nn.LayerNorm(4)))
+for call in (lambda: qnn.linear(torch.zeros(2, 4), torch.zeros(3, 4)), lambda: qnn.layer_norm(torch.zeros(2, 4), 4)):
+    try:
+        call()
+    except ImportError as e:
+        assert "no torch side" in str(e)
+    else:
+        raise AssertionError("not refused")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
+
+
+def test_torch_side_is_loaded_once():
+    import threading
+    from aimet_b200.v2 import nn as qnn
+    found = []
+    threads = [threading.Thread(target=lambda: found.append(qnn._layers)) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(found) == 8 and len({id(m) for m in found}) == 1 and callable(found[0].linear)
+    with pytest.raises(AttributeError):
+        qnn.no_such_name   # pylint: disable=pointless-statement

@@ -45,9 +45,29 @@ def needs_build(target: str = LIB_PATH, deps=None) -> bool:
     return any(os.path.getmtime(d) > t for d in deps + [os.path.abspath(__file__)])
 
 
+def _torch_tag() -> str:
+    """What the torch side's binary depends on beside its source."""
+    import torch
+    return f"torch {torch.__version__}, {sys.implementation.cache_tag}, cxx11 abi {int(torch.compiled_with_cxx11_abi())}"
+
+
+def _torch_tag_path() -> str:
+    return os.path.splitext(TORCH_PATH)[0] + ".built_for"
+
+
+def torch_side_is_foreign(unknown: bool = True) -> bool:
+    """Whether the torch side was built for another torch or Python than this one (its class layouts may differ);
+    ``unknown`` if nothing beside it says what it was built for."""
+    try:
+        with open(_torch_tag_path(), encoding="utf-8") as f:
+            return f.read() != _torch_tag()
+    except FileNotFoundError:
+        return unknown
+
+
 def build_torch(force: bool = False, verbose: bool = False) -> str:
     """The autograd functions of :mod:`aimet_b200.v2.nn`; against the torch that is installed."""
-    if not force and not needs_build(TORCH_PATH, [TORCH_SOURCE, os.path.join(CSRC, HEADERS[-1])]):
+    if not force and not needs_build(TORCH_PATH, [TORCH_SOURCE, os.path.join(CSRC, HEADERS[-1])]) and not torch_side_is_foreign():
         return TORCH_PATH
     import sysconfig
 
@@ -68,6 +88,8 @@ def build_torch(force: bool = False, verbose: bool = False) -> str:
         sys.stderr.write(res.stdout + res.stderr)
     if res.returncode != 0:
         raise RuntimeError("g++ failed building _torch_layers.so")
+    with open(_torch_tag_path(), "w", encoding="utf-8") as f:
+        f.write(_torch_tag())
     return TORCH_PATH
 
 

@@ -27,7 +27,7 @@ from typing import Optional, Sequence, Union
 import torch
 from torch import nn
 
-from .. import _lib
+from .. import _lib, build
 
 __all__ = ["linear", "layer_norm", "LayerNorm", "ACTIVATIONS", "wait_ran_out"]
 
@@ -35,7 +35,6 @@ __all__ = ["linear", "layer_norm", "LayerNorm", "ACTIVATIONS", "wait_ran_out"]
 ACTIVATIONS = {"relu": _lib.AQ_ACT_RELU, "gelu": _lib.AQ_ACT_GELU, "gelu_tanh": _lib.AQ_ACT_GELU_TANH,
                "silu": _lib.AQ_ACT_SILU}
 
-_TORCH_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lib", "_torch_layers.so")
 _ENTRIES = ("aq_status_string", "aq_last_cuda_error", "aq_align_rows", "aq_linear_forward",
             "aq_linear_grad_z_workspace_bytes", "aq_linear_grad_z", "aq_linear_grad_input", "aq_linear_grad_weight",
             "aq_layer_norm_forward", "aq_layer_norm_backward_workspace_bytes", "aq_layer_norm_backward")
@@ -43,9 +42,12 @@ _ENTRIES = ("aq_status_string", "aq_last_cuda_error", "aq_align_rows", "aq_linea
 
 def _load():
     """The compiled autograd functions (csrc/torch_layers.cpp), given the entry points of the loaded CUDA library."""
-    if not os.path.exists(_TORCH_PATH):
-        raise ImportError(f"{_TORCH_PATH} not found. Build it with `python -m aimet_b200.build`.")
-    spec = importlib.util.spec_from_file_location("_torch_layers", _TORCH_PATH)
+    path = build.TORCH_PATH
+    if not os.path.exists(path):
+        raise ImportError(f"{path} not found. Build it with `python -m aimet_b200.build`.")
+    if build.torch_side_is_foreign(unknown=False):
+        raise ImportError(f"{path} was built for another torch or Python. Build it with `python -m aimet_b200.build`.")
+    spec = importlib.util.spec_from_file_location("_torch_layers", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     module.bind({name: ctypes.cast(getattr(_lib.lib, name), ctypes.c_void_p).value for name in _ENTRIES})

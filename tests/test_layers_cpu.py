@@ -354,3 +354,30 @@ def test_torch_side_is_loaded_once():
     assert len(found) == 8 and len({id(m) for m in found}) == 1 and callable(found[0].linear)
     with pytest.raises(AttributeError):
         qnn.no_such_name   # pylint: disable=pointless-statement
+
+
+def test_torch_side_of_another_torch(monkeypatch, tmp_path):
+    """The torch side is rebuilt for, and not loaded into, a torch or a Python other than the one it was built for."""
+    import torch as installed
+    from aimet_b200 import build
+    from aimet_b200.v2 import nn as qnn
+    commands = []
+
+    def compiler(cmd, **_):
+        commands.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w", encoding="utf-8") as f:
+            f.write("library")
+        return type("Done", (), {"returncode": 0, "stdout": "", "stderr": ""})()
+
+    monkeypatch.setattr(build, "LIB_DIR", str(tmp_path))
+    monkeypatch.setattr(build, "TORCH_PATH", str(tmp_path / "_torch_layers.so"))
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    build.build_torch()
+    build.build_torch()
+    assert len(commands) == 1 and not build.torch_side_is_foreign()
+    monkeypatch.setattr(installed, "__version__", "9.9.9")
+    assert build.torch_side_is_foreign()
+    with pytest.raises(ImportError, match="another"):
+        qnn._load()
+    build.build_torch()
+    assert len(commands) == 2 and not build.torch_side_is_foreign()

@@ -437,10 +437,10 @@ __global__ void __launch_bounds__(128) few_rows_kernel(GemmArgs a)
     float v = mine;
     switch (a.act)
     {
-    case AQ_ACT_RELU: v = act_value<AQ_ACT_RELU>(v); break;
-    case AQ_ACT_GELU: v = act_value<AQ_ACT_GELU>(v); break;
-    case AQ_ACT_GELU_TANH: v = act_value<AQ_ACT_GELU_TANH>(v); break;
-    case AQ_ACT_SILU: v = act_value<AQ_ACT_SILU>(v); break;
+    case AQ_ACT_RELU: v = act_as<T, AQ_ACT_RELU>(v); break;
+    case AQ_ACT_GELU: v = act_as<T, AQ_ACT_GELU>(v); break;
+    case AQ_ACT_GELU_TANH: v = act_as<T, AQ_ACT_GELU_TANH>(v); break;
+    case AQ_ACT_SILU: v = act_as<T, AQ_ACT_SILU>(v); break;
     default: break;
     }
     if (a.residual)

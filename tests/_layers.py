@@ -140,3 +140,24 @@ def assert_within(got, ref, what=""):
         i = int(over.reshape(-1).argmax())
         raise AssertionError(f"{what}: element {i} is {float(got.reshape(-1)[i])!r}, want {float(want.reshape(-1)[i])!r} "
                              f"within {float(bound.reshape(-1)[i]):.3g}; {int((over > 0).sum())} of {got.numel()} are off")
+
+
+def norm_error(got, want):
+    """||got - want|| / ||want|| in float64."""
+    want = want.double()
+    return float((got.detach().double().reshape(want.shape) - want).norm() / want.norm())
+
+
+def float32_norm_bound(depth):
+    """What rounding leaves of a float32 sum of ``depth`` products of independent numbers around 0, over its norm.
+
+    After j products the sum is about sqrt(j) products large; rounding it is off by at most 2^-24 of that, with either sign:
+    sqrt(sum of j) = depth / sqrt(2) of them against sqrt(depth), so sqrt(depth / 2) 2^-24.  sqrt(depth) leaves room for
+    products that share a rounding; 4 more for the last steps.  Operands rounded to 10 bits are off by about 2^-12 each, for
+    every depth."""
+    return (math.sqrt(depth) + 4) * 2.0 ** -24
+
+
+FLOAT32_SIZES = [   # m, k, n: one row, few, 32-row tiles, 64 x 64, 128 x 128, with and without a split depth
+    (1, 4096, 512), (2, 64, 64), (8, 1000, 333), (31, 2048, 333), (65, 1001, 130), (200, 4000, 96), (128, 2048, 1000),
+    (512, 768, 768), (1100, 600, 1544), (1024, 1024, 1024)]

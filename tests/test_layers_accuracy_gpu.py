@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from _layers import TINY, U, act
+from _layers import FLOAT32_SIZES, TINY, U, act, float32_norm_bound, norm_error
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,17 @@ def test_gelu_of_negative_arguments(cuda, dtype, m, n):
     formula = (0.5 * z * poly * torch.exp(-z * z / 2) - want).abs()
     err = (y - want).abs() - (U[dtype] + 2.0 ** -16) * want.abs() - (1 + U[dtype]) * formula - TINY[dtype] / 2
     assert float(err.max()) <= 0, float((y - want).abs().div(want.abs()).max())
+
+
+@pytest.mark.parametrize("m,k,n", FLOAT32_SIZES)
+def test_float32_products_keep_their_operands(cuda, m, k, n):
+    """The three products of a float32 layer by their norms: operands of fewer bits would show at every depth."""
+    from aimet_b200.v2.nn import linear
+    g = torch.Generator(device="cuda").manual_seed(107)
+    x, w, dy = (torch.randn(s, device=cuda, generator=g).requires_grad_(True) for s in ((m, k), (n, k), (m, n)))
+    y = linear(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy.detach())
+    x, w, dy = x.detach().double(), w.detach().double(), dy.detach().double()
+    assert norm_error(y, x @ w.t()) <= float32_norm_bound(k)
+    assert norm_error(dx, dy @ w) <= float32_norm_bound(n)
+    assert norm_error(dw, dy.t() @ x) <= float32_norm_bound(m)

@@ -381,3 +381,22 @@ def test_torch_side_of_another_torch(monkeypatch, tmp_path):
         qnn._load()
     build.build_torch()
     assert len(commands) == 2 and not build.torch_side_is_foreign()
+
+
+@pytest.mark.parametrize("bits", [10, 7])
+def test_norm_bound_sees_operands_of_fewer_bits(bits):
+    """The check of the float32 products fails for operands rounded to 10 bits (7: bfloat16) at every size it is used at."""
+    from _layers import FLOAT32_SIZES, float32_norm_bound, norm_error
+    g = torch.Generator().manual_seed(109)
+
+    def cut(t):
+        mantissa, exponent = torch.frexp(t)
+        return torch.ldexp(torch.round(mantissa * 2 ** (bits + 1)) / 2 ** (bits + 1), exponent)
+
+    for m, k, n in FLOAT32_SIZES:
+        for depth, rows, cols in ((k, m, n), (n, m, k), (m, n, k)):
+            a, b = (torch.randn(s, generator=g, dtype=torch.float32).double() for s in ((rows, depth), (depth, cols)))
+            want = a @ b
+            assert norm_error(cut(a) @ cut(b), want) > 4 * float32_norm_bound(depth)
+            plain = (a.float() @ b.float()).double()
+            assert norm_error(plain, want) <= float32_norm_bound(depth)

@@ -1101,7 +1101,9 @@ int with_even_shape(int64_t packets, F&& f)
     AQ_SHAPE(512, 8)
     return AQ_ERR_TOO_LARGE;
 }
-// many rows of packets off 16-byte boundaries
+// Many rows of packets off 16-byte boundaries.  The shapes between the powers of two keep most of a CTA's threads on the row;
+// without them bf16, 2^26 elements: 2501 columns in 128 x 4 111 us, in 128 x 3 98; 5001 in 256 x 4 113, in 320 x 2 102; 6001 102
+// and in 384 x 2 94; 9001 in 512 x 4 145, in 320 x 4 119; 11001 125 and in 384 x 4 109.
 template <typename F>
 int with_any_shape(int64_t packets, F&& f)
 {
@@ -1133,8 +1135,11 @@ int with_short_shape(int64_t packets, F&& f)
     AQ_SHAPE(16, 4)
     return AQ_ERR_TOO_LARGE;
 }
-// the backward ring: 16 columns per thread where the row's length allows; a warp takes up to
-// 768 elements of 16 bits or 512 of 32 alone
+// The backward ring: 16 columns per thread where the row's length allows; a warp takes up to 768 elements of 16 bits or 512 of
+// 32 alone.  As above, backward pass with sums, 2^26 elements: bf16 600 columns in 128 threads 82 us, in a warp with three packets 67;
+// 11008 in 512 x 4 108, in 512 x 3 84 (float32 8500 in 512 x 8 157, in 512 x 6 138); off boundaries 5001 in 512 x 2 150, in
+// 320 x 2 121 (float32 4999 160 and 133).  192 threads for the rows between those of 128 and 256 were slower than 256 (bf16 2501
+// 181 and 144, float32 261 and 154).
 template <typename T, bool ANY, typename F>
 int with_sums_shape(int64_t packets, F&& f)
 {
@@ -1146,10 +1151,6 @@ int with_sums_shape(int64_t packets, F&& f)
         AQ_SHAPE(32, 3)
         AQ_SHAPE(128, 1)
         AQ_SHAPE(128, 2)
-        if constexpr (ANY)
-        {
-            AQ_SHAPE(192, 2)
-        }
         AQ_SHAPE(256, 2)
         if constexpr (ANY)
         {
@@ -1163,10 +1164,6 @@ int with_sums_shape(int64_t packets, F&& f)
     {
         AQ_SHAPE(32, 4)
         AQ_SHAPE(128, 4)
-        if constexpr (ANY)
-        {
-            AQ_SHAPE(192, 4)
-        }
         AQ_SHAPE(256, 4)
         if constexpr (ANY)
         {

@@ -454,7 +454,8 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& shape, const std:
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
     m.def("bind", &bind);
-    m.def("linear", &linear);
-    m.def("layer_norm", &layer_norm);
+    // without the interpreter's lock, as torch's own functions: a launch waits when the stream's queue is full
+    m.def("linear", &linear, py::call_guard<py::gil_scoped_release>());
+    m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
     m.def("rows_of", &rows_of);
 }

@@ -122,3 +122,51 @@ def test_norm_backward_from_two_threads(cuda):
 def test_no_wait_ran_out_here(cuda):
     from aimet_b200.v2.nn import wait_ran_out
     assert wait_ran_out() is False and wait_ran_out(cuda) is False
+
+
+def test_other_threads_run_while_launches_wait(cuda):
+    """A call whose launch waits for room in the stream's queue does not keep the interpreter's lock."""
+    import time
+    from aimet_b200.v2.nn import layer_norm, linear
+    x, w = torch.randn(4, 64, device=cuda), torch.randn(64, 64, device=cuda)
+    with torch.no_grad():
+        for fn in (lambda: linear(x, w), lambda: layer_norm(x, 64)):
+            fn()
+            torch.cuda.synchronize()
+            done = threading.Event()
+            gaps = []
+
+            def tick(done=done, gaps=gaps):
+                last = time.perf_counter()
+                while not done.is_set():
+                    time.sleep(0.001)
+                    now = time.perf_counter()
+                    gaps.append(now - last)
+                    last = now
+
+            t = threading.Thread(target=tick)
+            t.start()
+            start = time.perf_counter()
+            torch.cuda._sleep(1_000_000_000)   # about half a second; the queue fills after some 1000 launches
+            for _ in range(4000):
+                fn()
+            blocked = time.perf_counter() - start
+            done.set()
+            t.join()
+            torch.cuda.synchronize()
+            assert blocked > 0.3, "the queue never filled"
+            assert max(gaps) < 0.15, max(gaps)
+
+
+def test_saved_tensor_hooks_in_python(cuda):
+    """Code in Python that a call reaches: what packs and unpacks the tensors kept for the backward pass."""
+    from aimet_b200.v2.nn import layer_norm, linear
+    x = torch.randn(20, 64, device=cuda, requires_grad=True)
+    w = torch.randn(24, 64, device=cuda, requires_grad=True)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(tuple(t.shape)) or t.cpu(), lambda t: t.to(cuda)):
+        y = linear(layer_norm(x, 64), w, activation="gelu")
+    got = torch.autograd.grad(y.sum(), (x, w))
+    y = linear(layer_norm(x, 64), w, activation="gelu")
+    assert len(seen) >= 5
+    assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(y.sum(), (x, w))))

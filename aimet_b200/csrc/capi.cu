@@ -834,7 +834,10 @@ int aq_layers_stuck(int* h_out)
     if (!h_out)
         return AQ_ERR_INVALID_ARG;
     int gemm_flag = 0, norm_flag = 0;
-    int rc = gemm_stuck(&gemm_flag);
+    const cudaError_t e = cudaDeviceSynchronize();   // the copies below wait for the default stream alone
+    int rc              = e == cudaSuccess ? AQ_OK : cuda_fail(e);
+    if (rc == AQ_OK)
+        rc = gemm_stuck(&gemm_flag);
     if (rc == AQ_OK)
         rc = norm_stuck(&norm_flag);
     *h_out = gemm_flag || norm_flag;

@@ -548,7 +548,7 @@ int aq_linear_grad_weight(const void* d_dz, int64_t lddz, const void* d_x, int64
                           int dtype, int64_t m, int64_t n, int64_t k, void* stream);
 
 /* Every wait inside the layers' kernels is bounded (4 s).  *h_out: 0, or 1 once a wait has run out on the current
- * device since the library was loaded; the results concerned hold NaN.  Copies from the device (synchronises). */
+ * device since the library was loaded; the results concerned hold NaN.  Waits for the whole device. */
 int aq_layers_stuck(int* h_out);
 
 /* y = (x - mean) / sqrt(var + eps) * w + b over rows of dim elements (var: mean of squared differences).

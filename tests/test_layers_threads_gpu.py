@@ -170,3 +170,18 @@ def test_saved_tensor_hooks_in_python(cuda):
     y = linear(layer_norm(x, 64), w, activation="gelu")
     assert len(seen) >= 5
     assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(y.sum(), (x, w))))
+
+
+def test_wait_ran_out_waits_for_every_stream(cuda):
+    """torch's streams do not wait for the default one, nor it for them."""
+    from aimet_b200.v2.nn import linear, wait_ran_out
+    x, w = torch.randn(20, 64, device=cuda).half(), torch.randn(24, 64, device=cuda).half()
+    stream = torch.cuda.Stream()
+    linear(x, w)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)
+        linear(x, w)
+    assert not stream.query()
+    assert wait_ran_out() is False
+    assert stream.query()

@@ -171,8 +171,8 @@ def fuse_layers(gm: fx.GraphModule) -> int:
 
     A quantized ``nn.Linear`` becomes a :class:`QuantizedLinear`; a ReLU, GELU or SiLU that is its only consumer, and
     an addition of another tensor that is the only consumer of the result, move into its epilogue.  Whatever stands
-    between them -- an activation quantizer, a second consumer, a module with hooks -- keeps them apart, so the
-    placement of quantizers and what they see stay as they were.  ``nn.LayerNorm`` modules and ``F.layer_norm`` calls
+    between them -- an activation quantizer, a second consumer, a module with hooks, a write in place -- keeps them apart,
+    so the placement of quantizers and what they see stay as they were.  ``nn.LayerNorm`` modules and ``F.layer_norm`` calls
     are replaced too.  Returns the number of graph nodes that were replaced or taken in."""
     mods = dict(gm.named_modules())
     changed = 0
@@ -364,8 +364,11 @@ class QuantizationSimModel:
     def fuse_layers(self) -> int:
         """Runs the linear layers and layer norms of ``sim.model`` on the kernels of :mod:`aimet_b200.v2.nn`
         (:func:`fuse_layers`), with float32 sums in another order than torch's.  Quantizers, encodings and parameters
-        stay the same objects.  Can be called again, for instance after ``load_encodings(..., partial=False)`` removed
-        quantizers that kept a layer and its activation apart.  From then on the model needs CUDA tensors."""
+        stay the same objects.  The default placement has a quantizer behind every linear layer except before a ReLU:
+        until ``load_encodings(..., partial=False)`` has removed the quantizers that keep a layer, its activation and its
+        residual apart, only ReLUs move into the epilogue; call it again afterwards.  From then on the model needs CUDA
+        tensors of one dtype per layer, float32, float16 or bfloat16 (no autocast).  Meant for models in 16 bits: float32
+        products are slower than torch's."""
         changed = fuse_layers(self.model)
         self.layers = {name: self.model.get_submodule(name) for name in self.layers}
         return changed

@@ -18,6 +18,7 @@ from __future__ import annotations
 import contextlib
 import copy
 import operator
+import types
 from typing import Callable, Dict, List, Optional
 
 import torch
@@ -156,6 +157,9 @@ def _writes_in_place(node: fx.Node, mods: Dict[str, nn.Module]) -> bool:
     if node.op == "call_method":
         return node.target.endswith("_")
     if node.op == "call_function":
+        if isinstance(node.target, types.FunctionType) and \
+                (node.target.__module__ or "").partition(".")[0] not in ("torch", __name__.partition(".")[0]):
+            return True   # the user's own code (torch.fx.wrap), which may write to what it is given
         return (node.target in _IN_PLACE_FUNCS or getattr(node.target, "__name__", "").endswith("_") or
                 bool(node.kwargs.get("inplace")) or "out" in node.kwargs or
                 any(a is True for a in node.args[1:]))   # F.relu(x, True) and the like

@@ -247,6 +247,18 @@ def _between_activation_and_addition(s, x):
     return y + x
 
 
+@torch.fx.wrap
+def _doubled(h):
+    return h.mul_(2.0)
+
+
+def _wrapped_function_between(s, x):
+    h = x * 1.0
+    y = s.a(h)
+    g = _doubled(h)
+    return F.relu(y) * g
+
+
 @pytest.mark.parametrize("fn,mods,want", [
     (_mul_between, {}, [("linear", None, False)]),
     (_relu_between, {}, None),
@@ -254,6 +266,7 @@ def _between_activation_and_addition(s, x):
     (_function_between, {}, [("linear", None, False)]),
     (_dropout_between, {"g": nn.GELU()}, [("linear", None, False)]),
     (_between_activation_and_addition, {}, [("linear", "relu", False)]),
+    (_wrapped_function_between, {}, [("linear", None, False)]),
 ])
 def test_fuse_layers_reads_the_input_before_it_is_written(on_torch, fn, mods, want):
     """The layer's input is written in place before the activation (or the addition) is reached."""

@@ -155,7 +155,7 @@ def test_other_threads_run_while_launches_wait(cuda):
             t.join()
             torch.cuda.synchronize()
             assert blocked > 0.3, "the queue never filled"
-            assert max(gaps) < 0.15, max(gaps)
+            assert max(gaps) < 0.3, max(gaps)
 
 
 def test_saved_tensor_hooks_in_python(cuda):
@@ -180,7 +180,7 @@ def test_wait_ran_out_waits_for_every_stream(cuda):
     linear(x, w)
     torch.cuda.synchronize()
     with torch.cuda.stream(stream):
-        torch.cuda._sleep(200_000_000)
+        torch.cuda._sleep(1_000_000_000)
         linear(x, w)
     assert not stream.query()
     assert wait_ran_out() is False

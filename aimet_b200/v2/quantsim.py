@@ -153,13 +153,14 @@ _IN_PLACE_FUNCS = (operator.iadd, operator.isub, operator.imul, operator.itruedi
 
 def _writes_in_place(node: fx.Node, mods: Dict[str, nn.Module]) -> bool:
     if node.op == "call_module":
-        return bool(getattr(mods.get(node.target), "inplace", False))
+        m = mods.get(node.target)
+        return bool(getattr(m, "inplace", False)) or (m is not None and _has_hooks(m))   # a hook is the user's own code
     if node.op == "call_method":
         return node.target.endswith("_")
     if node.op == "call_function":
         if isinstance(node.target, types.FunctionType) and \
                 (node.target.__module__ or "").partition(".")[0] not in ("torch", __name__.partition(".")[0]):
-            return True   # the user's own code (torch.fx.wrap), which may write to what it is given
+            return True   # the same for torch.fx.wrap
         return (node.target in _IN_PLACE_FUNCS or getattr(node.target, "__name__", "").endswith("_") or
                 bool(node.kwargs.get("inplace")) or "out" in node.kwargs or
                 any(a is True for a in node.args[1:]))   # F.relu(x, True) and the like

@@ -413,3 +413,25 @@ def test_norm_bound_sees_operands_of_fewer_bits(bits):
             assert norm_error(cut(a) @ cut(b), want) > 4 * float32_norm_bound(depth)
             plain = (a.float() @ b.float()).double()
             assert norm_error(plain, want) <= float32_norm_bound(depth)
+
+
+def test_fuse_layers_keeps_its_order_around_hooks(on_torch):
+    """A hook of a module between the layer and its activation writes to the layer's input."""
+    def hooked_between(s, x):
+        h = x * 1.0
+        y = s.a(h)
+        g = s.i(h)
+        return F.relu(y) * g
+
+    torch.manual_seed(0)
+    net = _Net(hooked_between, i=nn.Identity()).eval()
+
+    def double(module, args):
+        args[0].mul_(2.0)
+
+    net.i.register_forward_pre_hook(double)
+    x = torch.randn(5, 8)
+    expect = net(x.clone())
+    sim, _ = _fused(net)
+    assert torch.allclose(sim.model(x.clone()), expect, atol=1e-6)
+    assert on_torch == [("linear", None, False)]
